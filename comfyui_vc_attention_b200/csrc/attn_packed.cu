@@ -1,0 +1,404 @@
+// Packed attention on register MMAs (mma.sync m16n8k16), for short query
+// sequences: every row of a KV head's group shares one pass over its keys.
+//
+//   O = softmax(scale q k^T + mask) v,  one pass with a running maximum m and
+//   sum l per row (both fp32):  O <- O 2^(m - m') + P V,  P = 2^(s - m')
+//
+// A tile is 64 rows (token, group head) of one sequence and KV head against a
+// range of its keys; four warps of 16 rows each share K and V tiles of 64 keys
+// that cp.async brings in two stages.  Keys past the sequence's end are filled
+// with zeros on the way in, so nothing of a neighbouring sequence (or of
+// unwritten memory) is multiplied.  A tile over part of the keys writes its
+// unnormalised rows, m and l; the join kernel adds the parts in key order.
+#include "attn_packed.cuh"
+
+#include <string>
+
+namespace vcattn {
+namespace {
+
+constexpr int kRows = 64;
+constexpr int kKeys = 64;
+constexpr int kWarps = 4;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// 16 bytes global -> shared; `bytes` of them read, the rest filled with zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == VCATTN_DTYPE_BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == VCATTN_DTYPE_BF16) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// Two 16-bit elements: is either infinite or NaN, and the pair with those set to 0.
+template <int DT> __device__ __forceinline__ uint32_t expo_mask() { return DT == VCATTN_DTYPE_BF16 ? 0x7f80u : 0x7c00u; }
+template <int DT> __device__ __forceinline__ bool bad2(uint32_t w) {
+  const uint32_t e = expo_mask<DT>();
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <int DT> __device__ __forceinline__ uint32_t clean2(uint32_t w) {
+  const uint32_t e = expo_mask<DT>();
+  if ((w & e) == e) w &= 0xffff0000u;
+  if (((w >> 16) & e) == e) w &= 0x0000ffffu;
+  return w;
+}
+template <int DT> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (DT == VCATTN_DTYPE_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <int D> struct Smem {
+  static constexpr int kPitch = D * 2 + 16;   // bytes: eight rows of a matrix start in different banks
+  static constexpr int kTile = kKeys * kPitch;
+  static constexpr int kBytes = 4 * kTile;    // K and V, two stages
+};
+
+template <int DT, int D>
+__device__ __forceinline__ void load_keys(uint32_t dst, const PackedArgs& a, const void* base, int64_t sh, int64_t sn,
+                                          const PackedTile& t, int head, int key0) {
+  const uint16_t* p = static_cast<const uint16_t*>(base) + head * sh;
+  for (int c = threadIdx.x; c < kKeys * (D / 8); c += kWarps * 32) {
+    const int r = c / (D / 8), ch = c % (D / 8);
+    const bool in = key0 + r < t.lk && t.k0 + key0 + r < a.Tk;
+    const int64_t row = in ? t.k0 + key0 + r : 0;
+    copy16(dst + r * Smem<D>::kPitch + ch * 16, p + row * sn + ch * 8, in ? 16 : 0);
+  }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  using S = Smem<D>;
+  const PackedTile t = a.tiles[blockIdx.x];
+  const int kvh = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+  const uint32_t s0 = smem_addr(smem);
+  const int n_rows = t.lq * a.G;
+
+  // this thread's two rows
+  int tok[2], head[2], lim[2];
+  bool live[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = t.r0 + warp * 16 + gid + 8 * i;
+    tok[i] = r / a.G;
+    head[i] = kvh * a.G + r - tok[i] * a.G;
+    live[i] = r < n_rows && t.q0 + tok[i] < a.Tq;
+    lim[i] = a.causal ? min(t.lk, tok[i] + t.lk - t.lq + 1) : t.lk;   // keys [0, lim) are seen
+    if (!live[i]) lim[i] = 0;
+  }
+  const int warp_tok = (t.r0 + warp * 16) / a.G;   // the first row sees the fewest keys
+  const int warp_lim = min(t.lk, warp_tok + t.lk - t.lq + 1);
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + (live[i] ? head[i] * a.qsh + (int64_t)(t.q0 + tok[i]) * a.qsn : 0);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qa[kk][i] = live[i] ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + tig * 2) : 0u;
+      qa[kk][2 + i] = live[i] ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 8 + tig * 2) : 0u;
+    }
+  }
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  const int steps = t.ke > t.kb ? (t.ke - t.kb + kKeys - 1) / kKeys : 0;
+  if (steps > 0) {
+    load_keys<DT, D>(s0, a, a.k, a.ksh, a.ksn, t, kvh, t.kb);
+    load_keys<DT, D>(s0 + S::kTile, a, a.v, a.vsh, a.vsn, t, kvh, t.kb);
+  }
+  copy_commit();
+  for (int j = 0; j < steps; ++j) {
+    const int key0 = t.kb + j * kKeys;
+    const uint32_t ks = s0 + (j & 1) * 2 * S::kTile, vs = ks + S::kTile;
+    if (j + 1 < steps) {
+      const uint32_t nx = s0 + ((j + 1) & 1) * 2 * S::kTile;
+      load_keys<DT, D>(nx, a, a.k, a.ksh, a.ksn, t, kvh, key0 + kKeys);
+      load_keys<DT, D>(nx + S::kTile, a, a.v, a.vsh, a.vsn, t, kvh, key0 + kKeys);
+    }
+    copy_commit();
+    copy_wait<1>();
+    __syncthreads();
+
+    float s[kKeys / 8][4];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; n += 2) {
+        // matrices: keys n*8.. (channels +0, +8), keys (n+1)*8.. (channels +0, +8)
+        uint32_t b[4];
+        ldsm4(b, ks + (n * 8 + (lane & 7) + ((lane >> 4) << 3)) * S::kPitch + kk * 32 + ((lane >> 3) & 1) * 16);
+        mma16<DT>(s[n], qa[kk], b[0], b[1]);
+        mma16<DT>(s[n + 1], qa[kk], b[2], b[3]);
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + n * 8 + tig * 2 + (e & 1), i = e >> 1;
+        s[n][e] = key < lim[i] ? s[n][e] * a.scale_log2 : -INFINITY;
+        mx[i] = fmaxf(mx[i], s[n][e]);
+      }
+    }
+    float base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      const float mn = fmaxf(m[i], mx[i]);
+      base[i] = mn == -INFINITY ? 0.f : mn;   // a row without a key so far
+      const float al = exp2f(m[i] - base[i]);
+      l[i] *= al;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][2 * i] *= al;
+        o[n][2 * i + 1] *= al;
+      }
+      m[i] = mn;
+    }
+    uint32_t pa[kKeys / 16][4];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = exp2f(s[n][e] - base[e >> 1]);
+        l[e >> 1] += p[e];
+      }
+      pa[n / 2][(n & 1) * 2] = pack2<DT>(p[0], p[1]);
+      pa[n / 2][(n & 1) * 2 + 1] = pack2<DT>(p[2], p[3]);
+    }
+    // Where the causal mask ends inside this tile, a row's masked keys have
+    // P = 0, but 0 times an infinite or NaN value is NaN.  If the tile holds
+    // such values, they enter the product as 0 and are added to the rows that
+    // do see them afterwards; the other rows' bits do not change.
+    bool bad = false;
+    if (a.causal && warp_lim < key0 + kKeys) {
+      for (int c = lane; c < kKeys * (D / 8); c += 32) {
+        const uint4 w = *reinterpret_cast<const uint4*>(smem + (vs - s0) + (c / (D / 8)) * S::kPitch + (c % (D / 8)) * 16);
+        bad |= bad2<DT>(w.x) || bad2<DT>(w.y) || bad2<DT>(w.z) || bad2<DT>(w.w);
+      }
+      bad = __any_sync(0xffffffffu, bad);
+    }
+#pragma unroll
+    for (int kk = 0; kk < kKeys / 16; ++kk) {
+#pragma unroll
+      for (int n = 0; n < D / 8; n += 2) {
+        uint32_t b[4];
+        ldsm4t(b, vs + (kk * 16 + (lane & 15)) * S::kPitch + n * 16 + (lane >> 4) * 16);
+        if (bad) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = clean2<DT>(b[e]);
+        }
+        mma16<DT>(o[n], pa[kk], b[0], b[1]);
+        mma16<DT>(o[n + 1], pa[kk], b[2], b[3]);
+      }
+    }
+    if (bad) {
+#pragma unroll
+      for (int n8 = 0; n8 < kKeys / 8; ++n8) {
+        for (int c = 0; c < 8; ++c) {   // key n8 * 8 + c: its P sits in lane c / 2 of the quad
+          const int key = n8 * 8 + c;
+          float p[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 f = unpack2<DT>(__shfl_sync(0xffffffffu, pa[n8 / 2][(n8 & 1) * 2 + i], (lane & 28) + (c >> 1)));
+            p[i] = (c & 1) ? f.y : f.x;
+          }
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + (vs - s0) + key * S::kPitch + n * 16 + tig * 4);
+            if (bad2<DT>(w)) {
+              const float2 f = unpack2<DT>(w);
+              const bool x = !isfinite(f.x), y = !isfinite(f.y);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                if (key0 + key < lim[i]) {
+                  if (x) o[n][2 * i] = fmaf(p[i], f.x, o[n][2 * i]);
+                  if (y) o[n][2 * i + 1] = fmaf(p[i], f.y, o[n][2 * i + 1]);
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (!live[i]) continue;
+    if (t.slot >= 0) {
+      const int64_t r = (static_cast<int64_t>(t.slot) * a.Hk + kvh) * kRows + warp * 16 + gid + 8 * i;
+      float* po = a.part_o + r * D + tig * 2;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(po + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+      if (tig == 0) *reinterpret_cast<float2*>(a.part_ml + r * 2) = make_float2(m[i], l[i]);
+    } else {
+      const float inv = lim[i] > 0 ? __fdiv_rn(1.f, l[i]) : 0.f;
+      uint16_t* p = static_cast<uint16_t*>(a.out) + head[i] * a.osh + static_cast<int64_t>(t.q0 + tok[i]) * a.osn + tig * 2;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<uint32_t*>(p + n * 8) =
+            lim[i] > 0 ? pack2<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv) : 0u;
+    }
+  }
+}
+
+// out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, one warp per row.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs a) {
+  const PackedJoin jn = a.joins[blockIdx.x / (kRows / 8)];
+  const int row = (blockIdx.x % (kRows / 8)) * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, lane = threadIdx.x & 31;
+  const int r = jn.r0 + row, tok = r / a.G;
+  if (r >= jn.lq * a.G || jn.q0 + tok >= a.Tq) return;
+  const int64_t step = static_cast<int64_t>(a.Hk) * kRows;
+  const int64_t first = (static_cast<int64_t>(jn.slot0) * a.Hk + kvh) * kRows + row;
+  float mx = -INFINITY;
+  for (int p = lane; p < jn.pieces; p += 32) mx = fmaxf(mx, a.part_ml[(first + p * step) * 2]);
+  mx = warp_max(mx);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  constexpr int C = D / 32;
+  float acc[C], den = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.f;
+  for (int p = 0; p < jn.pieces; ++p) {
+    const int64_t i = first + p * step;
+    const float w = exp2f(a.part_ml[i * 2] - base);
+    den = fmaf(w, a.part_ml[i * 2 + 1], den);
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = fmaf(w, a.part_o[i * D + lane * C + c], acc[c]);
+  }
+  const float inv = den != 0.f ? __fdiv_rn(1.f, den) : 0.f;
+  uint16_t* o = static_cast<uint16_t*>(a.out) + (kvh * a.G + r - tok * a.G) * a.osh + static_cast<int64_t>(jn.q0 + tok) * a.osn;
+#pragma unroll
+  for (int c = 0; c < C; c += 2)
+    *reinterpret_cast<uint32_t*>(o + lane * C + c) = mx == -INFINITY ? 0u : pack2<DT>(acc[c] * inv, acc[c + 1] * inv);
+}
+
+template <int DT, int D>
+cudaError_t launch(const PackedArgs& a, cudaStream_t st) {
+  auto k = attn_packed_kernel<DT, D>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes);
+  if (e != cudaSuccess) return e;
+  if (a.n_tiles > 0) {
+    k<<<dim3(a.n_tiles, a.Hk), kWarps * 32, Smem<D>::kBytes, st>>>(a);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess && a.n_joins > 0) {
+    attn_packed_join_kernel<DT, D><<<dim3(a.n_joins * (kRows / 8), a.Hk), 256, 0, st>>>(a);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+int arg_error(const char* msg) {
+  return record_error(VCATTN_ERR_ARG, (std::string("vcattn_attn_packed: ") + msg).c_str());
+}
+
+bool rows_fit(const vcattn_bhnd* v) {
+  return v != nullptr && v->data != nullptr && (reinterpret_cast<uintptr_t>(v->data) & 15u) == 0 && v->sh % 8 == 0 &&
+         v->sn % 8 == 0;
+}
+
+}  // namespace
+}  // namespace vcattn
+
+extern "C" {
+
+VCATTN_API size_t vcattn_attn_packed_workspace_bytes(int slots, int Hk, int D) {
+  if (slots <= 0 || Hk <= 0 || D <= 0) return 0;
+  return static_cast<size_t>(slots) * Hk * vcattn::kRows * (D + 2) * sizeof(float);
+}
+
+VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, const vcattn_bhnd* v, int dtype, int Hq,
+                                  int Hk, int Tq, int Tk, int D, const vcattn_packed_tile* tiles, int n_tiles,
+                                  const vcattn_packed_join* joins, int n_joins, int slots, int causal, float scale,
+                                  const vcattn_bhnd* out, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace vcattn;
+  static_assert(sizeof(PackedTile) == sizeof(vcattn_packed_tile) && sizeof(PackedJoin) == sizeof(vcattn_packed_join),
+                "the C ABI's records are the kernels'");
+  clear_error();
+  if (fault_injected("vcattn_attn_packed"))
+    return record_error(VCATTN_ERR_INJECTED, "vcattn_attn_packed: injected fault");
+  if (dtype != VCATTN_DTYPE_BF16 && dtype != VCATTN_DTYPE_F16) return arg_error("dtype must be bf16 or f16");
+  if (D != 64 && D != 128) return arg_error("D must be 64 or 128");
+  if (Hq <= 0 || Hk <= 0 || Hq % Hk || Hk > 65535) return arg_error("Hq must be a positive multiple of Hk");
+  if (Tq < 0 || Tk < 0 || n_tiles < 0 || n_joins < 0 || slots < 0) return arg_error("negative size");
+  if (!(scale > 0.f) || scale > 1e30f) return arg_error("scale must be positive and finite");
+  if (Tq == 0 || n_tiles == 0) return VCATTN_OK;
+  if (!tiles || (n_joins > 0 && !joins)) return arg_error("null pointer");
+  if (!rows_fit(q) || !rows_fit(out) || (Tk > 0 && (!rows_fit(k) || !rows_fit(v))))
+    return arg_error("q, k, v and out must be 16-byte aligned with strides of 16-byte multiples");
+  if (slots > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
+                    workspace_bytes < vcattn_attn_packed_workspace_bytes(slots, Hk, D)))
+    return record_error(VCATTN_ERR_WORKSPACE, "vcattn_attn_packed: workspace too small");
+  PackedArgs a{};
+  a.q = q->data; a.out = const_cast<void*>(out->data);
+  a.qsh = q->sh; a.qsn = q->sn; a.osh = out->sh; a.osn = out->sn;
+  if (Tk > 0) {
+    a.k = k->data; a.v = v->data;
+    a.ksh = k->sh; a.ksn = k->sn; a.vsh = v->sh; a.vsn = v->sn;
+  }
+  a.tiles = reinterpret_cast<const PackedTile*>(tiles);
+  a.joins = reinterpret_cast<const PackedJoin*>(joins);
+  a.n_tiles = n_tiles; a.n_joins = n_joins;
+  a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.Tq = Tq; a.Tk = Tk;
+  a.causal = causal ? 1 : 0;
+  a.scale_log2 = scale * kLog2e;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + static_cast<size_t>(slots) * Hk * kRows * D;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e =
+      dtype == VCATTN_DTYPE_BF16
+          ? (D == 128 ? launch<VCATTN_DTYPE_BF16, 128>(a, st) : launch<VCATTN_DTYPE_BF16, 64>(a, st))
+          : (D == 128 ? launch<VCATTN_DTYPE_F16, 128>(a, st) : launch<VCATTN_DTYPE_F16, 64>(a, st));
+  if (e != cudaSuccess)
+    return record_error(VCATTN_ERR_CUDA, (std::string("vcattn_attn_packed: ") + cudaGetErrorString(e)).c_str());
+  return VCATTN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,41 @@
+// Packed (ragged) attention: what the kernels and the entry point share.
+#pragma once
+
+#include "kernels.cuh"
+
+namespace vcattn {
+
+// One unit of work of a packed batch (32 bytes; vcattn_packed_tile in the C
+// ABI).  Rows are the sequence's (token, group head) pairs, row = token * G +
+// g, or its tokens, depending on the kernel.
+struct PackedTile {
+  int q0, lq;   // first query row of the sequence in the packed buffer, queries
+  int k0, lk;   // same for the keys
+  int r0;       // first row of this tile
+  int kb, ke;   // keys [kb, ke) of the sequence (empty: the output rows are 0)
+  int slot;     // index of its partial result, or -1: writes the output itself
+};
+
+// A group of partial results that join into one tile's output rows.
+struct PackedJoin {
+  int q0, lq, r0;
+  int slot0, pieces;
+  int unused[3];
+};
+
+struct PackedArgs {
+  const void *q, *k, *v;
+  void* out;
+  int64_t qsh, qsn, ksh, ksn, vsh, vsn, osh, osn;   // strides in elements over heads and rows
+  const PackedTile* tiles;
+  const PackedJoin* joins;
+  int n_tiles, n_joins;
+  int Hq, Hk, G, D;
+  int Tq, Tk;      // rows of the packed buffers: no tile reads or writes past them
+  int causal;
+  float scale_log2;   // softmax scale * log2(e)
+  float* part_o;      // [slot][kv head][rows][D]
+  float* part_ml;     // [slot][kv head][rows][2]: maximum (log2 domain) and sum
+};
+
+}  // namespace vcattn

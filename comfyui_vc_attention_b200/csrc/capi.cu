@@ -463,6 +463,13 @@ int vcattn_attn_status(int* code, int* where, int* block, int reset) {
     *where = 300 + w4;   // and those of the tensor-core k-means assignment as 300 + site
     *block = b4;
   }
+  int c5 = 0, w5 = 0, b5 = 0;
+  if (e == cudaSuccess) e = matmul_blocks_status(&c5, &w5, &b5, reset != 0);
+  if (e == cudaSuccess && *code == 0 && c5 != 0) {
+    *code = c5;
+    *where = 400 + w5;   // and those of the block-scaled FP8 product as 400 + site
+    *block = b5;
+  }
   return cuda_status(e, "vcattn_attn_status");
 }
 

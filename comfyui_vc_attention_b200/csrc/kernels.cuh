@@ -113,4 +113,11 @@ cudaError_t launch_codecs_fp4(const float* x, int64_t n, uint8_t* out, cudaStrea
 cudaError_t launch_expcast(const float* s, const float* m, int rows, int cols, double beta, int mode,
                            uint8_t* out, cudaStream_t st);
 
+// Error text and host fault injection of the C entry points (capi.cu), for
+// entry points that live beside their kernels.
+int record_error(int code, const char* msg);
+void clear_error();
+bool fault_injected(const char* entry_point);
+cudaError_t matmul_blocks_status(int* code, int* where, int* block, bool reset);
+
 }  // namespace vcattn

@@ -1,0 +1,361 @@
+// E4M3 matrix product with block scales, fp32 result rounded once:
+//   C[m, n] = sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in kb} A[m, k] B[n, k]  (+ bias[n])
+// with kb running over blocks of 128 columns (the last one may be short).
+//
+// tcgen05 kind::f8f6f4: each k-block of 128 is one accumulation of four MMAs in
+// tensor memory, in one of two buffers; the promotion warps read the finished
+// block sum and add it to fp32 registers with its scale while the next block
+// runs.  Thread = output row (TMEM lane), so the scale of a block is one
+// scalar per thread and 128 columns.
+#include <cuda.h>
+#include <mutex>
+#include <string>
+
+#include "kernels.cuh"
+#include "tc_common.cuh"
+#include "tc_math.cuh"
+
+namespace vcattn {
+
+__device__ tc::DevStatus g_matmul_status;
+
+namespace {
+
+using namespace tc;
+
+constexpr int kBM = 128;
+constexpr int kBK = 128;
+
+struct MatmulArgs {
+  const float *sa, *sb;
+  int64_t sam, sak, sbn, sbk;
+  const float* bias;
+  void* out;
+  int64_t ldo;
+  int M, N, kb;
+  int mt, nt, tiles, group;
+  int vec_out;   // rows of `out` start on 16-byte boundaries
+};
+
+template <int BN> struct MmCfg {
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kPromo = BN / 128;                  // promotion warpgroups
+  static constexpr int kThreads = 128 + 128 * kPromo;
+  static constexpr int kTmemCols = 2 * BN;
+};
+
+template <int BN> struct MmSmem {
+  alignas(1024) uint8_t a[MmCfg<BN>::kStages][kBM * kBK];
+  alignas(1024) uint8_t b[MmCfg<BN>::kStages][BN * kBK];
+  alignas(8) uint64_t full[MmCfg<BN>::kStages];
+  alignas(8) uint64_t empty[MmCfg<BN>::kStages];
+  alignas(8) uint64_t t_full[2];
+  alignas(8) uint64_t t_empty[2];
+  alignas(8) uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+// Tile t of the launch order: groups of `group` row tiles, rows fastest, so the
+// tiles that run together share their A and B panels in L2.
+__device__ __forceinline__ void tile_coords(const MatmulArgs& a, int t, int& m, int& n) {
+  const int per = a.group * a.nt;
+  const int g = t / per, r = t - g * per;
+  const int rows = min(a.group, a.mt - g * a.group);
+  n = r / rows;
+  m = g * a.group + (r - n * rows);
+}
+
+template <int BN, int ODT>
+__global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
+    matmul_blocks_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                         const MatmulArgs a) {
+  using Cfg = MmCfg<BN>;
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  MmSmem<BN>& sm = *reinterpret_cast<MmSmem<BN>*>(smem_raw + pad);
+  DevStatus* status = &g_matmul_status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    sm.abort = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.t_full[b], 1);
+      mbar_init(&sm.t_empty[b], 4 * Cfg::kPromo);
+    }
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = sm.tmem_base;
+  volatile int* abort = &sm.abort;
+  // BN = 256 is launched at 168 x 384 = 64512 registers: 128 x 40 + 256 x 232
+
+  if (warp < 4) {
+  if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n" ::: "memory");
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      prefetch_tmap(&tm_a);
+      prefetch_tmap(&tm_b);
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+        int m, n;
+        tile_coords(a, t, m, n);
+        for (int k = 0; k < a.kb; ++k, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && !(ok = mbar_wait(&sm.empty[s], ((it / kStages) + 1) & 1, abort, status, 1))) break;
+          mbar_expect_tx(&sm.full[s], (kBM + BN) * kBK);
+          tma_load_2d(sm.a[s], &tm_a, k * kBK, m * kBM, &sm.full[s]);
+          tma_load_2d(sm.b[s], &tm_b, k * kBK, n * BN, &sm.full[s]);
+        }
+      }
+      // on an abandoned run, let the copies already issued land
+      if (!ok || *abort) {
+        for (int j = max(0, it - kStages); j < it; ++j) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&sm.full[j % kStages], (j / kStages) & 1) && clock64() - t0 < kWaitCycles / 4) {
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t leader = elect_one();
+    const uint32_t idesc = idesc_e4m3(kBM, BN, false);
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+      for (int k = 0; k < a.kb; ++k, ++it) {
+        const int s = it % kStages, b = it & 1;
+        if (it >= 2 && !(ok = mbar_wait(&sm.t_empty[b], ((it >> 1) + 1) & 1, abort, status, 2))) break;
+        if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, abort, status, 3))) break;
+        tc_fence_after();
+        const uint32_t aa = smem_u32(sm.a[s]), ba = smem_u32(sm.b[s]);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_f8_if(tbase + b * BN, desc_kmajor(aa + kk * 32), desc_kmajor(ba + kk * 32), idesc, kk > 0, leader);
+        tc_commit_if(&sm.t_full[b], leader);
+        tc_commit_if(&sm.empty[s], leader);
+      }
+    }
+    // every MMA issued must finish before tensor memory is released
+    tc_commit_if(&sm.drain, leader);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(&sm.drain, 0) && clock64() - t0 < kWaitCycles) {
+    }
+    __syncwarp();
+  }
+  } else {
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n" ::: "memory");
+    // ------------------------------------------------------------ promotion and output
+    const int wq = warp & 3, col_half = (warp - 4) >> 2;
+    const uint32_t lb = tbase + (static_cast<uint32_t>(wq * 32) << 16) + col_half * 128;
+    constexpr int ES = ODT == VCATTN_DTYPE_F32 ? 4 : 2;
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+      int mt, nt;
+      tile_coords(a, t, mt, nt);
+      const int m = mt * kBM + wq * 32 + lane;
+      const int n0 = nt * BN + col_half * 128;
+      const bool live = m < a.M && n0 < a.N;
+      const float* sa = a.sa + static_cast<int64_t>(live ? m : 0) * a.sam;
+      const float* sb = a.sb + static_cast<int64_t>(live ? n0 / 128 : 0) * a.sbn;
+      float acc[128];
+#pragma unroll
+      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
+      float s_next = __ldg(sa) * __ldg(sb);
+      for (int k = 0; k < a.kb; ++k, ++it) {
+        const int b = it & 1;
+        const float s = s_next;
+        if (k + 1 < a.kb) s_next = __ldg(sa + (k + 1) * a.sak) * __ldg(sb + (k + 1) * a.sbk);
+        if (!(ok = mbar_wait(&sm.t_full[b], (it >> 1) & 1, abort, status, 4))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          float x[32];
+          tmem_ld32(lb + b * BN + h * 32, x);
+          tmem_ld_wait();
+          reg_fence(x);
+          if (h == 3) {
+            tc_fence_before();
+            warp_arrive(&sm.t_empty[b], lane);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) fma2(acc[h * 32 + c], acc[h * 32 + c + 1], x[c], x[c + 1], s, s);
+        }
+      }
+      if (!ok || *abort || !live) continue;
+      const int cols = min(128, a.N - n0);
+      uint8_t* o = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(m) * a.ldo + n0) * ES;
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 16 / ES) {
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 16 / ES; ++e)
+            if (c0 + e < cols) acc[c0 + e] += __ldg(a.bias + n0 + c0 + e);
+        }
+        if (a.vec_out && c0 + 16 / ES <= cols) {
+          uint4 w;
+#pragma unroll
+          for (int e = 0; e < 16 / ES; e += 2)
+            stage2<ODT>(reinterpret_cast<uint8_t*>(&w) + e * ES, acc[c0 + e], acc[c0 + e + 1]);
+          *reinterpret_cast<uint4*>(o + c0 * ES) = w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16 / ES; ++e) {
+            if (c0 + e < cols) {
+              if constexpr (ODT == VCATTN_DTYPE_BF16)
+                reinterpret_cast<__nv_bfloat16*>(o)[c0 + e] = __float2bfloat16_rn(acc[c0 + e]);
+              else if constexpr (ODT == VCATTN_DTYPE_F16)
+                reinterpret_cast<__half*>(o)[c0 + e] = __float2half_rn(acc[c0 + e]);
+              else
+                reinterpret_cast<float*>(o)[c0 + e] = acc[c0 + e];
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tbase, Cfg::kTmemCols);
+}
+
+// ---- host side ---------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// (rows, K) bytes, row pitch ld, box of box_rows x 128 columns in the 128-byte swizzle; outside reads 0.
+bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {kBK, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n > 0 ? n : 148;
+}
+
+struct Operands {
+  const uint8_t *a, *b;
+  int64_t lda, ldb, K;
+};
+
+template <int BN, int ODT>
+cudaError_t launch(const Operands& op, MatmulArgs a, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, op.a, a.M, op.K, op.lda, kBM) || !make_map(&mb, op.b, a.N, op.K, op.ldb, BN))
+    return cudaErrorInvalidValue;
+  a.mt = (a.M + kBM - 1) / kBM;
+  a.nt = (a.N + BN - 1) / BN;
+  a.tiles = a.mt * a.nt;
+  a.group = 16;
+  auto k = matmul_blocks_kernel<BN, ODT>;
+  const int smem = static_cast<int>(sizeof(MmSmem<BN>)) + 1024;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  k<<<static_cast<unsigned>(min(a.tiles, sm_count())), MmCfg<BN>::kThreads, smem, st>>>(ma, mb, a);
+  return cudaGetLastError();
+}
+
+template <int ODT>
+cudaError_t dispatch(const Operands& op, const MatmulArgs& a, cudaStream_t st) {
+  // 256-column tiles halve the A traffic per MMA; with too few tiles to fill
+  // the SMs the narrower tile spreads the work further.
+  const int64_t wide = static_cast<int64_t>((a.M + 127) / 128) * ((a.N + 255) / 256);
+  return wide >= sm_count() ? launch<256, ODT>(op, a, st) : launch<128, ODT>(op, a, st);
+}
+
+int arg_error(const char* msg) {
+  return record_error(VCATTN_ERR_ARG, (std::string("vcattn_matmul_blocks: ") + msg).c_str());
+}
+
+}  // namespace
+
+cudaError_t matmul_blocks_status(int* code, int* where, int* block, bool reset) {
+  tc::DevStatus s{};
+  cudaError_t e = cudaMemcpyFromSymbol(&s, g_matmul_status, sizeof(s));
+  if (e != cudaSuccess) return e;
+  *code = s.code;
+  *where = s.where;
+  *block = s.block;
+  if (reset) {
+    tc::DevStatus z{};
+    e = cudaMemcpyToSymbol(g_matmul_status, &z, sizeof(z));
+  }
+  return e;
+}
+
+}  // namespace vcattn
+
+extern "C" VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float* a_scale, int64_t as_m,
+                                               int64_t as_k, const uint8_t* b8, int64_t ldb, const float* b_scale,
+                                               int64_t bs_n, int64_t bs_k, int64_t M, int64_t N, int64_t K,
+                                               const float* bias, void* out, int out_dtype, int64_t ldo,
+                                               void* stream) {
+  using namespace vcattn;
+  clear_error();
+  if (fault_injected("vcattn_matmul_blocks"))
+    return record_error(VCATTN_ERR_INJECTED, "vcattn_matmul_blocks: injected fault");
+  if (out_dtype != VCATTN_DTYPE_BF16 && out_dtype != VCATTN_DTYPE_F16 && out_dtype != VCATTN_DTYPE_F32)
+    return arg_error("unsupported output dtype");
+  if (M < 0 || N < 0 || K <= 0 || M > (int64_t{1} << 30) || N > (int64_t{1} << 30) || K > (int64_t{1} << 30))
+    return arg_error("size out of range");
+  if (M == 0 || N == 0) return VCATTN_OK;
+  if (!a8 || !a_scale || !b8 || !b_scale || !out) return arg_error("null pointer");
+  if ((reinterpret_cast<uintptr_t>(a8) & 15u) || (reinterpret_cast<uintptr_t>(b8) & 15u) || lda % 16 || ldb % 16 ||
+      lda < K || ldb < K)
+    return arg_error("code rows must be 16-byte aligned, with a pitch of at least K that is a multiple of 16");
+  if (ldo < N) return arg_error("output row stride below N");
+  if ((M + 127) / 128 * ((N + 127) / 128) >= (int64_t{1} << 31)) return arg_error("more than 2^31 tiles");
+  const int es = out_dtype == VCATTN_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % es) return arg_error("misaligned output");
+  MatmulArgs a{};
+  a.sa = a_scale; a.sam = as_m; a.sak = as_k; a.sb = b_scale; a.sbn = bs_n; a.sbk = bs_k;
+  a.bias = bias; a.out = out; a.ldo = ldo; a.M = static_cast<int>(M); a.N = static_cast<int>(N);
+  a.kb = static_cast<int>((K + kBK - 1) / kBK);
+  a.vec_out = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (ldo * es) % 16 == 0;
+  const Operands op{a8, b8, lda, ldb, K};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = out_dtype == VCATTN_DTYPE_BF16  ? dispatch<VCATTN_DTYPE_BF16>(op, a, st)
+                        : out_dtype == VCATTN_DTYPE_F16 ? dispatch<VCATTN_DTYPE_F16>(op, a, st)
+                                                        : dispatch<VCATTN_DTYPE_F32>(op, a, st);
+  if (e != cudaSuccess)
+    return record_error(VCATTN_ERR_CUDA, (std::string("vcattn_matmul_blocks: ") + cudaGetErrorString(e)).c_str());
+  return VCATTN_OK;
+}

@@ -35,6 +35,8 @@ SMOOTH_K = 2
 V_MMA_ORDER = 4
 EXPCAST = 1
 EXPCAST_EXACT = 2
+ROPE_INTERLEAVED = 1
+ROPE_NORM = 2
 
 
 class NativeUnavailable(RuntimeError):
@@ -116,6 +118,18 @@ _SIGNATURES = {
                                           c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
                                           c_double, c_void_p, c_int, c_int64, c_int64, c_int64,
                                           c_void_p]),
+    "vcattn_qk_norm_rope": (c_int, [POINTER(BHND), POINTER(BHND), c_int, c_int, c_int, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int,
+                                    c_float, POINTER(BHND), POINTER(BHND), c_void_p]),
+    "vcattn_quantize_blocks": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64,
+                                       c_void_p, c_int64, c_int64, c_void_p]),
+    "vcattn_matmul_blocks": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,
+                                     c_int64, c_void_p]),
+    "vcattn_attn_packed_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vcattn_attn_packed": (c_int, [POINTER(BHND), POINTER(BHND), POINTER(BHND), c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float, POINTER(BHND),
+                                   c_void_p, c_size_t, c_void_p]),
     "vcattn_e4m3_encode": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "vcattn_fp4_encode": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "vcattn_expcast_codes": (c_int, [c_void_p, c_void_p, c_int, c_int, c_double, c_int, c_void_p,

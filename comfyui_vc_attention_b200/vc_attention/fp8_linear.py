@@ -1,0 +1,138 @@
+"""8-bit linear layers: E4M3 codes with one scale for each block of 128.
+
+Activations are quantised per (row, 128 columns), weights per (128 x 128), and
+the product applies both scales to each block's partial sum in fp32::
+
+    w = quantize_blocks(weight, rows=128)          # once
+    y = linear_blocks(x, w, bias)                  # quantize_blocks(x) + matmul_blocks
+
+Kernels: ``vcattn_quantize_blocks`` and ``vcattn_matmul_blocks`` (tcgen05).
+Forward only.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native as N
+from ._launch import on_device, refuse_grad, stream
+from .grouping import _dtype_code
+
+__all__ = ["Fp8Blocks", "quantize_blocks", "matmul_blocks", "linear_blocks"]
+
+BLOCK = 128
+
+
+class Fp8Blocks(NamedTuple):
+    """A quantised (M, K) matrix: value = codes * scale of its block."""
+    codes: torch.Tensor   # (M, K) float8_e4m3fn, row pitch a multiple of 16
+    scale: torch.Tensor   # (ceil(M / rows), ceil(K / 128)) fp32
+    rows: int             # 1 or 128 rows per block
+
+
+def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Fp8Blocks:
+    """E4M3 codes and scales of x, (M, K) or (..., K) with the leading
+    dimensions flattened; CUDA bf16 / fp16 / fp32.
+
+    rows=1: a scale per row and 128 columns (activations); rows=128: per
+    128 x 128 block (weights).  scale = max(max |x|, 1e-30) / 448, codes =
+    E4M3(x / scale), round to nearest even.  The scales are stored with rows
+    side by side (the order the product reads them in).
+    """
+    refuse_grad("quantize_blocks", x)
+    if not x.is_cuda:
+        raise RuntimeError("quantize_blocks needs a CUDA tensor (this build has no CPU path)")
+    if rows not in (1, BLOCK):
+        raise ValueError(f"rows must be 1 or {BLOCK}, got {rows}")
+    dt = _dtype_code(x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must be (M, K) with K > 0, got {tuple(x.shape)}")
+    k = x.shape[-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    m = x2.shape[0]
+    if x2.stride(1) != 1 or (m > 1 and x2.stride(0) < k):
+        x2 = x2.contiguous()
+    ldx = x2.stride(0) if m > 1 else k
+    ldc = -(-k // 16) * 16
+    codes = torch.empty((m, ldc), dtype=torch.float8_e4m3fn, device=x.device)
+    if ldc != k:
+        codes = codes[:, :k]
+    kb = -(-k // BLOCK)
+    scale = torch.empty((kb, -(-m // rows)), dtype=torch.float32, device=x.device)
+    with on_device(x.device):
+        N.check("vcattn_quantize_blocks", N.lib().vcattn_quantize_blocks(
+            x2.data_ptr(), dt, m, k, ldx, rows, codes.data_ptr(), ldc, scale.data_ptr(), 1, scale.shape[1], stream(x.device)))
+    return Fp8Blocks(codes, scale.t(), rows)
+
+
+def _check_blocks(b: Fp8Blocks, name: str, rows: int):
+    if not (b.codes.is_cuda and b.scale.is_cuda) or b.codes.device != b.scale.device:
+        raise RuntimeError(f"matmul_blocks needs CUDA tensors on one device ({name})")
+    if b.rows != rows:
+        raise ValueError(f"{name} must have one scale per {rows} row(s) and {BLOCK} columns, got rows={b.rows}")
+    if b.codes.dtype != torch.float8_e4m3fn or b.codes.dim() != 2 or b.codes.shape[1] == 0:
+        raise ValueError(f"{name}.codes must be (rows, K) float8_e4m3fn, got {tuple(b.codes.shape)} {b.codes.dtype}")
+    m, k = b.codes.shape
+    want = (-(-m // rows), -(-k // BLOCK))
+    if b.scale.dtype != torch.float32 or tuple(b.scale.shape) != want:
+        raise ValueError(f"{name}.scale must be {want} float32, got {tuple(b.scale.shape)} {b.scale.dtype}")
+
+
+def _code_rows(c: torch.Tensor):
+    """(tensor, row pitch): codes as the TMA reads them (16-byte rows), copied if need be."""
+    m, k = c.shape
+    ld = c.stride(0) if m > 1 else -(-k // 16) * 16
+    if c.stride(1) == 1 and c.data_ptr() % 16 == 0 and ld % 16 == 0 and ld >= k:
+        return c, ld
+    ld = -(-k // 16) * 16
+    t = torch.empty((m, ld), dtype=c.dtype, device=c.device)
+    t[:, :k].copy_(c)
+    return t, ld
+
+
+def matmul_blocks(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
+                  dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """a @ b.T (+ bias): (M, K) x (N, K) -> (M, N) in ``dtype``.
+
+    a has rows=1 (activations), b rows=128 (weights); each product of 128
+    columns is scaled by both blocks' scales and added in fp32, and the result
+    is rounded once.  bias: (N,) or None.  out: (M, N) of ``dtype`` with
+    contiguous columns, or None.
+    """
+    _check_blocks(a, "a", 1)
+    _check_blocks(b, "b", BLOCK)
+    refuse_grad("matmul_blocks", a.scale, b.scale, bias)
+    m, k = a.codes.shape
+    n = b.codes.shape[0]
+    dev = a.codes.device
+    if b.codes.shape[1] != k or b.codes.device != dev:
+        raise ValueError(f"a and b must share K and a device, got {tuple(a.codes.shape)} on {dev}, "
+                         f"{tuple(b.codes.shape)} on {b.codes.device}")
+    if bias is not None:
+        if bias.shape != (n,) or bias.device != dev:
+            raise ValueError(f"bias must be ({n},) on {dev}, got {tuple(bias.shape)} on {bias.device}")
+        bias = bias.to(torch.float32).contiguous()
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    elif out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or \
+            (m > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be ({m}, {n}) {dtype} on {dev} with contiguous columns")
+    odt = _dtype_code(out)
+    ac, lda = _code_rows(a.codes)
+    bc, ldb = _code_rows(b.codes)
+    ldo = out.stride(0) if m > 1 else max(n, 1)
+    with on_device(dev):
+        N.check("vcattn_matmul_blocks", N.lib().vcattn_matmul_blocks(
+            ac.data_ptr(), lda, a.scale.data_ptr(), a.scale.stride(0), a.scale.stride(1),
+            bc.data_ptr(), ldb, b.scale.data_ptr(), b.scale.stride(0), b.scale.stride(1), m, n, k,
+            None if bias is None else bias.data_ptr(), out.data_ptr(), odt, ldo, stream(dev)))
+    return out
+
+
+def linear_blocks(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] = None,
+                  dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x (..., K) times a quantised (N, K) weight: (..., N) in ``dtype`` (x's by default)."""
+    y = matmul_blocks(quantize_blocks(x), weight, bias, dtype or x.dtype)
+    return y.view(*x.shape[:-1], y.shape[-1])

@@ -1,0 +1,159 @@
+"""Exact attention over packed sequences of different lengths.
+
+The rows VC-Attention leaves to an exact kernel -- text prompts and refiner
+blocks, prompt encoders (causal, grouped heads), sequences below
+``min_tokens``, single new tokens against their history -- lie one after the
+other in one buffer.  ``packed_plan`` lays the batch out once (the lengths are
+host numbers, checked here, so no call can read past the buffers) and
+``packed_attention`` runs it for every layer.
+
+Kernel: ``vcattn_attn_packed``.  Forward only.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import _native as N
+from ._launch import on_device, out_rows, refuse_grad, stream, view
+from .grouping import _dtype_code
+
+__all__ = ["PackedPlan", "packed_plan", "packed_attention"]
+
+TILE_ROWS = 64      # rows (token, group head) of a tile
+KEY_STEP = 64       # keys a tile takes at a time
+SPLIT_KEYS = 256    # shortest key range worth a tile of its own
+
+
+@dataclass(frozen=True)
+class PackedPlan:
+    """Work of one batch layout, on the device (made by ``packed_plan``)."""
+    heads: int
+    kv_heads: int
+    head_dim: int
+    causal: bool
+    total_q: int
+    total_k: int
+    tiles: torch.Tensor     # (n, 8) int32 records of vcattn_packed_tile
+    joins: torch.Tensor     # (n, 8) int32 records of vcattn_packed_join
+    slots: int              # partial results
+
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.device
+
+
+def _lengths(x, what) -> np.ndarray:
+    a = np.asarray([int(v) for v in x], dtype=np.int64)
+    if (a < 0).any():
+        raise ValueError(f"{what} must not be negative")
+    if a.sum() >= 2 ** 31:
+        raise ValueError(f"{what} add up to 2^31 rows or more")
+    return a
+
+
+def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, heads: int,
+                kv_heads: Optional[int] = None, head_dim: int, causal: bool = False,
+                device: Optional[torch.device] = None) -> PackedPlan:
+    """Lay out a batch: sequence i has q_lens[i] queries and k_lens[i] keys
+    (default: as many), the rows of sequence i + 1 following those of i.
+
+    causal: query t of lq sees keys up to t + lk - lq (the last query sees
+    every key, as when lq new tokens follow a history); a query before the
+    first key sees none and its output is 0.  heads must be a multiple of
+    kv_heads (default: heads); head_dim is 64 or 128.
+    """
+    kv_heads = heads if kv_heads is None else kv_heads
+    ql = _lengths(q_lens, "q_lens")
+    kl = ql if k_lens is None else _lengths(k_lens, "k_lens")
+    if len(ql) != len(kl):
+        raise ValueError(f"{len(ql)} query lengths and {len(kl)} key lengths")
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"heads ({heads}) must be a positive multiple of kv_heads ({kv_heads})")
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+    g = heads // kv_heads
+    if (ql * g >= 2 ** 31).any():
+        raise ValueError("a sequence has 2^31 rows or more")
+    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    q0, k0 = np.cumsum(ql) - ql, np.cumsum(kl) - kl
+
+    # tiles of TILE_ROWS rows, each with the keys its last token sees
+    per = -(-(ql * g) // TILE_ROWS)
+    seq = np.repeat(np.arange(len(ql)), per)
+    r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * TILE_ROWS
+    lq, lk = ql[seq], kl[seq]
+    last = np.minimum((r0 + TILE_ROWS - 1) // g, lq - 1)
+    ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk.copy()
+    # a batch that leaves SMs idle splits its longest key ranges
+    pieces = np.ones(len(seq), dtype=np.int64)
+    work = int(ke.sum()) * kv_heads
+    if len(seq) * kv_heads < 4 * 148 and work:
+        share = max(SPLIT_KEYS, -(-work // (4 * 148)))
+        pieces = np.maximum(1, -(-ke // share))
+    span = -(-(-(-ke // pieces)) // KEY_STEP) * KEY_STEP     # keys per piece
+    pieces = np.maximum(1, -(-ke // np.maximum(span, 1)))
+    n = int(pieces.sum())
+    row = np.repeat(np.arange(len(seq)), pieces)
+    piece = np.arange(n) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+    kb = piece * span[row]
+    split = pieces[row] > 1
+    slot = np.where(split, np.cumsum(split) - 1, -1)
+    tiles = np.stack([q0[seq][row], lq[row], k0[seq][row], lk[row], r0[row], kb,
+                      np.minimum(kb + span[row], ke[row]), slot], axis=1).astype(np.int32)
+    tiles = tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")]   # longest first
+    js = np.nonzero(pieces > 1)[0]
+    first = np.cumsum(np.where(pieces > 1, pieces, 0)) - np.where(pieces > 1, pieces, 0)
+    joins = np.zeros((len(js), 8), dtype=np.int32)
+    joins[:, 0], joins[:, 1], joins[:, 2] = q0[seq][js], lq[js], r0[js]
+    joins[:, 3], joins[:, 4] = first[js], pieces[js]
+    put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), put(tiles), put(joins),
+                      int(split.sum()))
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T + mask) v for every sequence of ``plan``.
+
+    q: (1, heads, total_q, D), k, v: (1, kv_heads, total_k, D) CUDA bf16 or
+    fp16 views (channels contiguous; others are copied).  scale: positive,
+    default D ** -0.5.  Returns (1, heads, total_q, D) in q's token layout, or
+    writes ``out``.  Scores, statistics and sums are fp32; P is rounded to q's
+    type for the second product.
+    """
+    refuse_grad("packed_attention", q, k, v)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError("packed_attention needs CUDA tensors (this build has no CPU path)")
+    d = plan.head_dim
+    want_q, want_k = (1, plan.heads, plan.total_q, d), (1, plan.kv_heads, plan.total_k, d)
+    if q.shape != want_q or k.shape != want_k or v.shape != want_k:
+        raise ValueError(f"the plan needs q {want_q} and k, v {want_k}, got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k, v must share bfloat16 or float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if not q.device == k.device == v.device == plan.device:
+        raise ValueError("q, k, v and the plan must be on one device")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    out = out_rows(out, q, "out")
+    if plan.total_q == 0:
+        return out
+    (qv, q), (kv, k), (vv, v), (ov, _) = view(q), view(k), view(v), view(out)
+    lib = N.lib()
+    ws, ws_bytes = None, 0
+    if plan.slots:
+        ws_bytes = lib.vcattn_attn_packed_workspace_bytes(plan.slots, plan.kv_heads, d)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    with on_device(q.device):
+        N.check("vcattn_attn_packed", lib.vcattn_attn_packed(
+            qv, kv, vv, _dtype_code(q), plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d,
+            plan.tiles.data_ptr(), plan.tiles.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.slots,
+            int(plan.causal), scale, ov, None if ws is None else ws.data_ptr(), ws_bytes,
+            stream(q.device)))
+    return out

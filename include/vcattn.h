@@ -52,6 +52,10 @@ extern "C" {
 #define VCATTN_DTYPE_F16 1
 #define VCATTN_DTYPE_F32 2
 
+/* ---- flags of vcattn_qk_norm_rope ---------------------------------------- */
+#define VCATTN_ROPE_INTERLEAVED 1  /* rotate channel pairs (2i, 2i+1), not (i, i + rot/2) */
+#define VCATTN_ROPE_NORM 2         /* RMS norm of each head row before the rotation     */
+
 /* ---- prepare flags (triton_attn.py:504-512 hadamard / smooth_k) --------- */
 #define VCATTN_HADAMARD 1
 #define VCATTN_SMOOTH_K 2
@@ -326,6 +330,74 @@ VCATTN_API int vcattn_attn_fp8_sparse_tc(const uint8_t* q8, const float* q_scale
                               float sm_scale, int flags, double expcast_beta,
                               void* out, int out_dtype, int64_t out_sb, int64_t out_sh,
                               int64_t out_sn, void* stream);
+
+/* ---- per-head RMS norm of Q and K with the position rotation, one pass ------
+ *   y = x * rsqrt(mean_d x^2 + eps) * w        (VCATTN_ROPE_NORM)
+ *   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s) on the first `rot` channels,
+ * j = i + rot/2, or j = i + 1 for even i (VCATTN_ROPE_INTERLEAVED).  q and
+ * q_out are (B, Hq, N, D) views, k and k_out (B, Hk, N, D); an output may be
+ * its input.  cos_table / sin_table: fp32 (B or 1, N, rot/2) with element
+ * strides table_sb (0: shared by the batch) and table_sn, channels contiguous.
+ * Weights (D,) fp32 or NULL (ones).  D a multiple of 8 up to 256, rot a
+ * multiple of 16 up to D (0: no rotation, tables may be NULL). */
+VCATTN_API int vcattn_qk_norm_rope(const vcattn_bhnd* q, const vcattn_bhnd* k, int dtype, int B, int Hq, int Hk,
+                        int N, int D, const float* q_weight, const float* k_weight,
+                        const float* cos_table, const float* sin_table, int64_t table_sb,
+                        int64_t table_sn, int rot, int flags, float eps,
+                        const vcattn_bhnd* q_out, const vcattn_bhnd* k_out, void* stream);
+
+/* ---- E4M3 quantisation with a scale for each block of 128 columns -----------
+ *   s = max(max |x|, 1e-30) / 448 over block_rows x 128 elements,
+ *   code = E4M3(x / s)
+ * x (M, K) of `dtype` with row stride ldx; block_rows 1 (activations) or 128
+ * (weights).  codes (M, K) bytes, row pitch ldc (a multiple of 16); scale fp32
+ * (ceil(M / block_rows), ceil(K / 128)) with element strides scale_sm and
+ * scale_sk. */
+VCATTN_API int vcattn_quantize_blocks(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int block_rows,
+                           uint8_t* codes, int64_t ldc, float* scale, int64_t scale_sm, int64_t scale_sk,
+                           void* stream);
+
+/* ---- E4M3 matrix product with block scales ----------------------------------
+ *   out[m, n] = sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in kb} a[m, k] b[n, k] (+ bias[n])
+ * a (M, K) and b (N, K) E4M3 codes with row pitches lda, ldb (multiples of 16,
+ * 16-byte aligned); a_scale (M, ceil(K/128)) and b_scale (ceil(N/128),
+ * ceil(K/128)) fp32 with element strides; bias (N,) fp32 or NULL.  fp32 sums,
+ * one rounding to out_dtype.  Bounded waits report through
+ * vcattn_attn_status as 400 + site. */
+VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float* a_scale, int64_t as_m, int64_t as_k,
+                         const uint8_t* b8, int64_t ldb, const float* b_scale, int64_t bs_n, int64_t bs_k,
+                         int64_t M, int64_t N, int64_t K, const float* bias, void* out, int out_dtype,
+                         int64_t ldo, void* stream);
+
+/* ---- exact attention over packed sequences ----------------------------------
+ * Sequences of different lengths lie one after the other in q / out
+ * ((1, Hq, Tq, D) views; sb unused) and k / v ((1, Hk, Tk, D)); Hq a multiple
+ * of Hk, D in {64, 128}, bf16 or f16.  causal != 0: query i of lq sees keys
+ * [0, i + 1 + lk - lq) (the last query sees every key).  A row that sees no
+ * key gives 0.  P is rounded to the input type for the P V product, sums and
+ * statistics are fp32.
+ * The host lays the work out once per batch as device arrays of records (rows
+ * are (token, group head) pairs, row = token * Hq/Hk + g, 64 per tile):
+ * tiles, and for sequences whose keys are split over several tiles, `slots`
+ * partial results and the joins that add them up.  Records that point past
+ * Tq or Tk are cut there. */
+typedef struct vcattn_packed_tile {
+  int32_t q0, lq;   /* first query row in the packed buffer, queries   */
+  int32_t k0, lk;   /* first key row, keys                             */
+  int32_t r0;       /* first row of the tile                           */
+  int32_t kb, ke;   /* keys [kb, ke) of the sequence                   */
+  int32_t slot;     /* partial result, or -1: writes out itself        */
+} vcattn_packed_tile;
+typedef struct vcattn_packed_join {
+  int32_t q0, lq, r0;        /* as in the tiles that it joins          */
+  int32_t slot0, pieces;     /* partial results [slot0, slot0 + pieces) */
+  int32_t unused[3];
+} vcattn_packed_join;
+VCATTN_API size_t vcattn_attn_packed_workspace_bytes(int slots, int Hk, int D);
+VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, const vcattn_bhnd* v, int dtype, int Hq,
+                       int Hk, int Tq, int Tk, int D, const vcattn_packed_tile* tiles, int n_tiles,
+                       const vcattn_packed_join* joins, int n_joins, int slots, int causal, float scale,
+                       const vcattn_bhnd* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- element codecs, exposed for bit-exact tests ------------------------
  * vcattn_e4m3_encode: quant.py:56-84.  vcattn_fp4_encode: quant.py:144-161
