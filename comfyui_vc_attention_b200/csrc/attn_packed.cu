@@ -17,7 +17,7 @@
 namespace vcattn {
 namespace {
 
-constexpr int kRows = 64;
+constexpr int kRows = kPackedRows;
 constexpr int kKeys = 64;
 constexpr int kWarps = 4;
 
@@ -278,25 +278,26 @@ __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedAr
       for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(po + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
       if (tig == 0) *reinterpret_cast<float2*>(a.part_ml + r * 2) = make_float2(m[i], l[i]);
     } else {
-      const float inv = lim[i] > 0 ? __fdiv_rn(1.f, l[i]) : 0.f;
+      const float inv = l[i] != 0.f ? __fdiv_rn(1.f, l[i]) : 0.f;   // no key, no output
       uint16_t* p = static_cast<uint16_t*>(a.out) + head[i] * a.osh + static_cast<int64_t>(t.q0 + tok[i]) * a.osn + tig * 2;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<uint32_t*>(p + n * 8) =
-            lim[i] > 0 ? pack2<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv) : 0u;
+        *reinterpret_cast<uint32_t*>(p + n * 8) = pack2<DT>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
     }
   }
 }
 
-// out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, one warp per row.
-template <int DT, int D>
-__global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs a) {
-  const PackedJoin jn = a.joins[blockIdx.x / (kRows / 8)];
-  const int row = (blockIdx.x % (kRows / 8)) * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, lane = threadIdx.x & 31;
-  const int r = jn.r0 + row, tok = r / a.G;
-  if (r >= jn.lq * a.G || jn.q0 + tok >= a.Tq) return;
-  const int64_t step = static_cast<int64_t>(a.Hk) * kRows;
-  const int64_t first = (static_cast<int64_t>(jn.slot0) * a.Hk + kvh) * kRows + row;
+// out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, one warp per row.  The
+// parts of a tile of R rows belong to `heads` heads; row = token * G + g is
+// query head head * G + g.
+template <int DT, int D, int R>
+__global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs a, int heads, int G) {
+  const PackedJoin jn = a.joins[blockIdx.x / (R / 8)];
+  const int row = (blockIdx.x % (R / 8)) * 8 + (threadIdx.x >> 5), head = blockIdx.y, lane = threadIdx.x & 31;
+  const int r = jn.r0 + row, tok = r / G;
+  if (tok >= jn.lq || jn.q0 + tok >= a.Tq) return;
+  const int64_t step = static_cast<int64_t>(heads) * R;
+  const int64_t first = (static_cast<int64_t>(jn.slot0) * heads + head) * R + row;
   float mx = -INFINITY;
   for (int p = lane; p < jn.pieces; p += 32) mx = fmaxf(mx, a.part_ml[(first + p * step) * 2]);
   mx = warp_max(mx);
@@ -313,24 +314,32 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs 
     for (int c = 0; c < C; ++c) acc[c] = fmaf(w, a.part_o[i * D + lane * C + c], acc[c]);
   }
   const float inv = den != 0.f ? __fdiv_rn(1.f, den) : 0.f;
-  uint16_t* o = static_cast<uint16_t*>(a.out) + (kvh * a.G + r - tok * a.G) * a.osh + static_cast<int64_t>(jn.q0 + tok) * a.osn;
+  uint16_t* o = static_cast<uint16_t*>(a.out) + (head * G + r - tok * G) * a.osh + static_cast<int64_t>(jn.q0 + tok) * a.osn;
 #pragma unroll
-  for (int c = 0; c < C; c += 2)
-    *reinterpret_cast<uint32_t*>(o + lane * C + c) = mx == -INFINITY ? 0u : pack2<DT>(acc[c] * inv, acc[c + 1] * inv);
+  for (int c = 0; c < C; c += 2) *reinterpret_cast<uint32_t*>(o + lane * C + c) = pack2<DT>(acc[c] * inv, acc[c + 1] * inv);
+}
+
+template <int DT, int D, int R>
+cudaError_t join(const PackedArgs& a, int heads, int G, cudaStream_t st) {
+  if (a.n_joins == 0) return cudaSuccess;
+  attn_packed_join_kernel<DT, D, R><<<dim3(a.n_joins * (R / 8), heads), 256, 0, st>>>(a, heads, G);
+  return cudaGetLastError();
 }
 
 template <int DT, int D>
-cudaError_t launch(const PackedArgs& a, cudaStream_t st) {
-  auto k = attn_packed_kernel<DT, D>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes);
-  if (e != cudaSuccess) return e;
-  if (a.n_tiles > 0) {
-    k<<<dim3(a.n_tiles, a.Hk), kWarps * 32, Smem<D>::kBytes, st>>>(a);
-    e = cudaGetLastError();
+cudaError_t launch(const PackedArgs& narrow, const PackedArgs& wide, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  if (wide.n_tiles > 0) {
+    e = launch_attn_packed_tc(wide, DT, st);
+    if (e == cudaSuccess) e = join<DT, D, kPackedWideRows>(wide, wide.Hq, 1, st);
   }
-  if (e == cudaSuccess && a.n_joins > 0) {
-    attn_packed_join_kernel<DT, D><<<dim3(a.n_joins * (kRows / 8), a.Hk), 256, 0, st>>>(a);
+  if (e == cudaSuccess && narrow.n_tiles > 0) {
+    auto k = attn_packed_kernel<DT, D>;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes);
+    if (e != cudaSuccess) return e;
+    k<<<dim3(narrow.n_tiles, narrow.Hk), kWarps * 32, Smem<D>::kBytes, st>>>(narrow);
     e = cudaGetLastError();
+    if (e == cudaSuccess) e = join<DT, D, kPackedRows>(narrow, narrow.Hk, narrow.G, st);
   }
   return e;
 }
@@ -349,15 +358,17 @@ bool rows_fit(const vcattn_bhnd* v) {
 
 extern "C" {
 
-VCATTN_API size_t vcattn_attn_packed_workspace_bytes(int slots, int Hk, int D) {
-  if (slots <= 0 || Hk <= 0 || D <= 0) return 0;
-  return static_cast<size_t>(slots) * Hk * vcattn::kRows * (D + 2) * sizeof(float);
+VCATTN_API size_t vcattn_attn_packed_workspace_bytes(const vcattn_packed_work* work, int Hq, int Hk, int D) {
+  if (work == nullptr || work->slots < 0 || work->wide_slots < 0 || Hq <= 0 || Hk <= 0 || D <= 0) return 0;
+  const size_t rows = static_cast<size_t>(work->slots) * Hk * vcattn::kPackedRows +
+                      static_cast<size_t>(work->wide_slots) * Hq * vcattn::kPackedWideRows;
+  return rows * (D + 2) * sizeof(float);
 }
 
 VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, const vcattn_bhnd* v, int dtype, int Hq,
-                                  int Hk, int Tq, int Tk, int D, const vcattn_packed_tile* tiles, int n_tiles,
-                                  const vcattn_packed_join* joins, int n_joins, int slots, int causal, float scale,
-                                  const vcattn_bhnd* out, void* workspace, size_t workspace_bytes, void* stream) {
+                                  int Hk, int Tq, int Tk, int D, const vcattn_packed_work* work, int causal,
+                                  float scale, const vcattn_bhnd* out, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   using namespace vcattn;
   static_assert(sizeof(PackedTile) == sizeof(vcattn_packed_tile) && sizeof(PackedJoin) == sizeof(vcattn_packed_join),
                 "the C ABI's records are the kernels'");
@@ -366,15 +377,21 @@ VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, co
     return record_error(VCATTN_ERR_INJECTED, "vcattn_attn_packed: injected fault");
   if (dtype != VCATTN_DTYPE_BF16 && dtype != VCATTN_DTYPE_F16) return arg_error("dtype must be bf16 or f16");
   if (D != 64 && D != 128) return arg_error("D must be 64 or 128");
-  if (Hq <= 0 || Hk <= 0 || Hq % Hk || Hk > 65535) return arg_error("Hq must be a positive multiple of Hk");
-  if (Tq < 0 || Tk < 0 || n_tiles < 0 || n_joins < 0 || slots < 0) return arg_error("negative size");
+  if (Hq <= 0 || Hk <= 0 || Hq % Hk || Hq > 65535) return arg_error("Hq must be a positive multiple of Hk, at most 65535");
+  if (!work) return arg_error("null pointer");
+  if (Tq < 0 || Tk < 0 || work->n_tiles < 0 || work->n_joins < 0 || work->slots < 0 || work->n_wide < 0 ||
+      work->n_wide_joins < 0 || work->wide_slots < 0)
+    return arg_error("negative size");
   if (!(scale > 0.f) || scale > 1e30f) return arg_error("scale must be positive and finite");
-  if (Tq == 0 || n_tiles == 0) return VCATTN_OK;
-  if (!tiles || (n_joins > 0 && !joins)) return arg_error("null pointer");
+  if (Tq == 0 || work->n_tiles + work->n_wide == 0) return VCATTN_OK;
+  if ((work->n_tiles > 0 && !work->tiles) || (work->n_joins > 0 && !work->joins) ||
+      (work->n_wide > 0 && !work->wide_tiles) || (work->n_wide_joins > 0 && !work->wide_joins))
+    return arg_error("null pointer");
+  if (static_cast<int64_t>(work->n_wide) * Hq >= (int64_t{1} << 31)) return arg_error("more than 2^31 tiles");
   if (!rows_fit(q) || !rows_fit(out) || (Tk > 0 && (!rows_fit(k) || !rows_fit(v))))
     return arg_error("q, k, v and out must be 16-byte aligned with strides of 16-byte multiples");
-  if (slots > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
-                    workspace_bytes < vcattn_attn_packed_workspace_bytes(slots, Hk, D)))
+  const size_t need = vcattn_attn_packed_workspace_bytes(work, Hq, Hk, D);
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < need))
     return record_error(VCATTN_ERR_WORKSPACE, "vcattn_attn_packed: workspace too small");
   PackedArgs a{};
   a.q = q->data; a.out = const_cast<void*>(out->data);
@@ -383,19 +400,26 @@ VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, co
     a.k = k->data; a.v = v->data;
     a.ksh = k->sh; a.ksn = k->sn; a.vsh = v->sh; a.vsn = v->sn;
   }
-  a.tiles = reinterpret_cast<const PackedTile*>(tiles);
-  a.joins = reinterpret_cast<const PackedJoin*>(joins);
-  a.n_tiles = n_tiles; a.n_joins = n_joins;
   a.Hq = Hq; a.Hk = Hk; a.G = Hq / Hk; a.D = D; a.Tq = Tq; a.Tk = Tk;
   a.causal = causal ? 1 : 0;
   a.scale_log2 = scale * kLog2e;
+  PackedArgs w = a;
+  a.tiles = reinterpret_cast<const PackedTile*>(work->tiles);
+  a.joins = reinterpret_cast<const PackedJoin*>(work->joins);
+  a.n_tiles = work->n_tiles; a.n_joins = work->n_joins;
+  const size_t rows = static_cast<size_t>(work->slots) * Hk * kPackedRows;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + static_cast<size_t>(slots) * Hk * kRows * D;
+  a.part_ml = a.part_o + rows * D;
+  w.tiles = reinterpret_cast<const PackedTile*>(work->wide_tiles);
+  w.joins = reinterpret_cast<const PackedJoin*>(work->wide_joins);
+  w.n_tiles = work->n_wide; w.n_joins = work->n_wide_joins;
+  w.part_o = a.part_ml + rows * 2;
+  w.part_ml = w.part_o + static_cast<size_t>(work->wide_slots) * Hq * kPackedWideRows * D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e =
       dtype == VCATTN_DTYPE_BF16
-          ? (D == 128 ? launch<VCATTN_DTYPE_BF16, 128>(a, st) : launch<VCATTN_DTYPE_BF16, 64>(a, st))
-          : (D == 128 ? launch<VCATTN_DTYPE_F16, 128>(a, st) : launch<VCATTN_DTYPE_F16, 64>(a, st));
+          ? (D == 128 ? launch<VCATTN_DTYPE_BF16, 128>(a, w, st) : launch<VCATTN_DTYPE_BF16, 64>(a, w, st))
+          : (D == 128 ? launch<VCATTN_DTYPE_F16, 128>(a, w, st) : launch<VCATTN_DTYPE_F16, 64>(a, w, st));
   if (e != cudaSuccess)
     return record_error(VCATTN_ERR_CUDA, (std::string("vcattn_attn_packed: ") + cudaGetErrorString(e)).c_str());
   return VCATTN_OK;

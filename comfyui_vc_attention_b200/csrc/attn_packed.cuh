@@ -23,6 +23,7 @@ struct PackedJoin {
   int unused[3];
 };
 
+// Arguments of one kernel over one list of tiles.
 struct PackedArgs {
   const void *q, *k, *v;
   void* out;
@@ -34,8 +35,15 @@ struct PackedArgs {
   int Tq, Tk;      // rows of the packed buffers: no tile reads or writes past them
   int causal;
   float scale_log2;   // softmax scale * log2(e)
-  float* part_o;      // [slot][kv head][rows][D]
-  float* part_ml;     // [slot][kv head][rows][2]: maximum (log2 domain) and sum
+  float* part_o;      // [slot][head][rows][D]
+  float* part_ml;     // [slot][head][rows][2]: reference (log2 domain) and sum
 };
+
+// Rows of a tile, and so of a partial result: (token, group head) pairs of one
+// KV head on register MMAs, tokens of one query head on tcgen05.
+constexpr int kPackedRows = 64;
+constexpr int kPackedWideRows = 256;
+
+cudaError_t launch_attn_packed_tc(const PackedArgs& a, int dtype, cudaStream_t st);
 
 }  // namespace vcattn

@@ -470,6 +470,13 @@ int vcattn_attn_status(int* code, int* where, int* block, int reset) {
     *where = 400 + w5;   // and those of the block-scaled FP8 product as 400 + site
     *block = b5;
   }
+  int c6 = 0, w6 = 0, b6 = 0;
+  if (e == cudaSuccess) e = attn_packed_status(&c6, &w6, &b6, reset != 0);
+  if (e == cudaSuccess && *code == 0 && c6 != 0) {
+    *code = c6;
+    *where = 500 + w6;   // and those of the packed attention kernel as 500 + site
+    *block = b6;
+  }
   return cuda_status(e, "vcattn_attn_status");
 }
 

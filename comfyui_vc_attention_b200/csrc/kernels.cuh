@@ -119,5 +119,6 @@ int record_error(int code, const char* msg);
 void clear_error();
 bool fault_injected(const char* entry_point);
 cudaError_t matmul_blocks_status(int* code, int* where, int* block, bool reset);
+cudaError_t attn_packed_status(int* code, int* where, int* block, bool reset);
 
 }  // namespace vcattn

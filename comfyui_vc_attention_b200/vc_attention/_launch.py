@@ -37,8 +37,9 @@ def rows_aligned(x: torch.Tensor) -> bool:
 
 
 def view(x: torch.Tensor) -> Tuple[N.BHND, torch.Tensor]:
-    """vcattn_bhnd of x and the tensor it points into (a copy if the rows are not aligned)."""
-    if not rows_aligned(x):
+    """vcattn_bhnd of x and the tensor it points into (a copy if the rows are
+    not aligned, or are the same memory as those of a broadcast view)."""
+    if not rows_aligned(x) or (0 in x.stride() and x.numel() > x.shape[-1]):
         x = x.clone(memory_format=torch.contiguous_format)
     sb, sh, sn, _ = x.stride()
     return N.BHND(x.data_ptr(), sb, sh, sn), x
@@ -59,6 +60,6 @@ def out_rows(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> torch.T
         return empty_like_rows(x)
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{what} must match its input: {tuple(x.shape)} {x.dtype} on {x.device}")
-    if out.numel() and not rows_aligned(out):
-        raise ValueError(f"{what} must have contiguous channels and 16-byte aligned rows")
+    if out.numel() and (not rows_aligned(out) or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape))):
+        raise ValueError(f"{what} must have contiguous channels and 16-byte aligned rows of their own")
     return out

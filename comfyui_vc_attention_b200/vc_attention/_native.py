@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_size_t,
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t,
                     c_uint8, c_void_p)
 from typing import Optional
 
@@ -61,6 +61,13 @@ class RouteStats(Structure):
     """vcattn_route_stats."""
     _fields_ = [("q_block", c_int), ("k_mean", c_void_p), ("q_cent", c_void_p),
                 ("q_bar", c_void_p), ("v_mean", c_void_p), ("sm_scale", c_float)]
+
+
+class PackedWork(Structure):
+    """vcattn_packed_work: the device records of a packed batch."""
+    _fields_ = [("tiles", c_void_p), ("joins", c_void_p), ("wide_tiles", c_void_p), ("wide_joins", c_void_p),
+                ("n_tiles", c_int32), ("n_joins", c_int32), ("slots", c_int32),
+                ("n_wide", c_int32), ("n_wide_joins", c_int32), ("wide_slots", c_int32)]
 
 
 _SIGNATURES = {
@@ -126,10 +133,10 @@ _SIGNATURES = {
     "vcattn_matmul_blocks": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                      c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,
                                      c_int64, c_void_p]),
-    "vcattn_attn_packed_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vcattn_attn_packed_workspace_bytes": (c_size_t, [POINTER(PackedWork), c_int, c_int, c_int]),
     "vcattn_attn_packed": (c_int, [POINTER(BHND), POINTER(BHND), POINTER(BHND), c_int, c_int, c_int, c_int, c_int,
-                                   c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float, POINTER(BHND),
-                                   c_void_p, c_size_t, c_void_p]),
+                                   c_int, POINTER(PackedWork), c_int, c_float, POINTER(BHND), c_void_p, c_size_t,
+                                   c_void_p]),
     "vcattn_e4m3_encode": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "vcattn_fp4_encode": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "vcattn_expcast_codes": (c_int, [c_void_p, c_void_p, c_int, c_int, c_double, c_int, c_void_p,

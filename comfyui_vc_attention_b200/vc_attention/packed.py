@@ -7,7 +7,8 @@ other in one buffer.  ``packed_plan`` lays the batch out once (the lengths are
 host numbers, checked here, so no call can read past the buffers) and
 ``packed_attention`` runs it for every layer.
 
-Kernel: ``vcattn_attn_packed``.  Forward only.
+Kernels: ``vcattn_attn_packed`` (tcgen05 for sequences of many queries,
+register MMAs over the rows of a KV head's group for few).  Forward only.
 """
 
 from __future__ import annotations
@@ -24,9 +25,14 @@ from .grouping import _dtype_code
 
 __all__ = ["PackedPlan", "packed_plan", "packed_attention"]
 
-TILE_ROWS = 64      # rows (token, group head) of a tile
-KEY_STEP = 64       # keys a tile takes at a time
-SPLIT_KEYS = 256    # shortest key range worth a tile of its own
+SMS = 148
+
+# Rows of a tile, keys it takes at a time, and the shortest key range worth a
+# tile of its own: register-MMA tiles of (token, group head) rows, and tcgen05
+# tiles of tokens.
+NARROW = (64, 64, 256)
+WIDE = (256, 128, 1024)
+WIDE_FROM = 64   # queries of a sequence that goes to the tcgen05 kernel
 
 
 @dataclass(frozen=True)
@@ -38,9 +44,12 @@ class PackedPlan:
     causal: bool
     total_q: int
     total_k: int
-    tiles: torch.Tensor     # (n, 8) int32 records of vcattn_packed_tile
-    joins: torch.Tensor     # (n, 8) int32 records of vcattn_packed_join
-    slots: int              # partial results
+    tiles: torch.Tensor         # (n, 8) int32 records of vcattn_packed_tile
+    joins: torch.Tensor         # (n, 8) int32 records of vcattn_packed_join
+    wide_tiles: torch.Tensor
+    wide_joins: torch.Tensor
+    work: N.PackedWork          # the four arrays for the C ABI
+    workspace_bytes: int        # partial results of one call
 
     @property
     def device(self) -> torch.device:
@@ -54,6 +63,39 @@ def _lengths(x, what) -> np.ndarray:
     if a.sum() >= 2 ** 31:
         raise ValueError(f"{what} add up to 2^31 rows or more")
     return a
+
+
+def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
+    """Tile and join records (int32 arrays) of the given sequences, and the
+    number of partial results.  A batch that would leave SMs idle splits its
+    longest key ranges."""
+    rows, step, least = shape
+    per = -(-(ql * group) // rows)
+    seq = np.repeat(np.arange(len(ql)), per)
+    r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * rows
+    lq, lk = ql[seq], kl[seq]
+    last = np.minimum((r0 + rows - 1) // group, lq - 1)
+    ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk.copy()
+    pieces = np.ones(len(seq), dtype=np.int64)
+    work = int(ke.sum()) * heads
+    slots = 4 * SMS if shape is NARROW else SMS
+    if len(seq) * heads < slots and work:
+        pieces = np.maximum(1, -(-ke // max(least, -(-work // slots))))
+    span = -(-(-(-ke // pieces)) // step) * step             # keys per piece
+    pieces = np.maximum(1, -(-ke // np.maximum(span, 1)))
+    row = np.repeat(np.arange(len(seq)), pieces)
+    piece = np.arange(len(row)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+    kb = piece * span[row]
+    split = pieces[row] > 1
+    slot = np.where(split, np.cumsum(split) - 1, -1)
+    tiles = np.stack([q0[seq][row], lq[row], k0[seq][row], lk[row], r0[row], kb,
+                      np.minimum(kb + span[row], ke[row]), slot], axis=1).astype(np.int32)
+    tiles = tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")]   # longest first
+    js = np.nonzero(pieces > 1)[0]
+    joins = np.zeros((len(js), 8), dtype=np.int32)
+    joins[:, 0], joins[:, 1], joins[:, 2] = q0[seq][js], lq[js], r0[js]
+    joins[:, 3], joins[:, 4] = np.cumsum(pieces[js]) - pieces[js], pieces[js]
+    return tiles, joins, int(split.sum())
 
 
 def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, heads: int,
@@ -81,39 +123,16 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
         raise ValueError("a sequence has 2^31 rows or more")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     q0, k0 = np.cumsum(ql) - ql, np.cumsum(kl) - kl
-
-    # tiles of TILE_ROWS rows, each with the keys its last token sees
-    per = -(-(ql * g) // TILE_ROWS)
-    seq = np.repeat(np.arange(len(ql)), per)
-    r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * TILE_ROWS
-    lq, lk = ql[seq], kl[seq]
-    last = np.minimum((r0 + TILE_ROWS - 1) // g, lq - 1)
-    ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk.copy()
-    # a batch that leaves SMs idle splits its longest key ranges
-    pieces = np.ones(len(seq), dtype=np.int64)
-    work = int(ke.sum()) * kv_heads
-    if len(seq) * kv_heads < 4 * 148 and work:
-        share = max(SPLIT_KEYS, -(-work // (4 * 148)))
-        pieces = np.maximum(1, -(-ke // share))
-    span = -(-(-(-ke // pieces)) // KEY_STEP) * KEY_STEP     # keys per piece
-    pieces = np.maximum(1, -(-ke // np.maximum(span, 1)))
-    n = int(pieces.sum())
-    row = np.repeat(np.arange(len(seq)), pieces)
-    piece = np.arange(n) - np.repeat(np.cumsum(pieces) - pieces, pieces)
-    kb = piece * span[row]
-    split = pieces[row] > 1
-    slot = np.where(split, np.cumsum(split) - 1, -1)
-    tiles = np.stack([q0[seq][row], lq[row], k0[seq][row], lk[row], r0[row], kb,
-                      np.minimum(kb + span[row], ke[row]), slot], axis=1).astype(np.int32)
-    tiles = tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")]   # longest first
-    js = np.nonzero(pieces > 1)[0]
-    first = np.cumsum(np.where(pieces > 1, pieces, 0)) - np.where(pieces > 1, pieces, 0)
-    joins = np.zeros((len(js), 8), dtype=np.int32)
-    joins[:, 0], joins[:, 1], joins[:, 2] = q0[seq][js], lq[js], r0[js]
-    joins[:, 3], joins[:, 4] = first[js], pieces[js]
+    wide = ql >= WIDE_FROM
+    parts = [_tiles(q0[s], ql[s], k0[s], kl[s], *how) for s, how in
+             ((~wide, (g, kv_heads, causal, NARROW)), (wide, (1, heads, causal, WIDE)))]
     put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
-    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), put(tiles), put(joins),
-                      int(split.sum()))
+    (tiles, joins, slots), (wtiles, wjoins, wslots) = ((put(t), put(j), s) for t, j, s in parts)
+    work = N.PackedWork(tiles.data_ptr(), joins.data_ptr(), wtiles.data_ptr(), wjoins.data_ptr(), tiles.shape[0],
+                        joins.shape[0], slots, wtiles.shape[0], wjoins.shape[0], wslots)
+    need = (slots * kv_heads * NARROW[0] + wslots * heads * WIDE[0]) * (head_dim + 2) * 4
+    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), tiles, joins, wtiles,
+                      wjoins, work, need)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,
@@ -145,15 +164,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     if plan.total_q == 0:
         return out
     (qv, q), (kv, k), (vv, v), (ov, _) = view(q), view(k), view(v), view(out)
-    lib = N.lib()
-    ws, ws_bytes = None, 0
-    if plan.slots:
-        ws_bytes = lib.vcattn_attn_packed_workspace_bytes(plan.slots, plan.kv_heads, d)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device) if plan.workspace_bytes else None
     with on_device(q.device):
-        N.check("vcattn_attn_packed", lib.vcattn_attn_packed(
-            qv, kv, vv, _dtype_code(q), plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d,
-            plan.tiles.data_ptr(), plan.tiles.shape[0], plan.joins.data_ptr(), plan.joins.shape[0], plan.slots,
-            int(plan.causal), scale, ov, None if ws is None else ws.data_ptr(), ws_bytes,
+        N.check("vcattn_attn_packed", N.lib().vcattn_attn_packed(
+            qv, kv, vv, _dtype_code(q), plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d, plan.work,
+            int(plan.causal), scale, ov, None if ws is None else ws.data_ptr(), plan.workspace_bytes,
             stream(q.device)))
     return out

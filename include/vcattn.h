@@ -376,11 +376,15 @@ VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float*
  * [0, i + 1 + lk - lq) (the last query sees every key).  A row that sees no
  * key gives 0.  P is rounded to the input type for the P V product, sums and
  * statistics are fp32.
- * The host lays the work out once per batch as device arrays of records (rows
- * are (token, group head) pairs, row = token * Hq/Hk + g, 64 per tile):
- * tiles, and for sequences whose keys are split over several tiles, `slots`
- * partial results and the joins that add them up.  Records that point past
- * Tq or Tk are cut there. */
+ * Strides of k and v may not be 0 over a dimension of more than one.
+ * The host lays the work out once per batch as device arrays of records.
+ * `tiles` run on register MMAs: 64 rows of one KV head, row = token * Hq/Hk +
+ * g; `wide_tiles` run on tcgen05: 256 rows of one query head, row = token.
+ * Every query row belongs to one tile, or to the tiles of one join where its
+ * keys are split over several; those write `slots` partial results that the
+ * joins add up in key order.  kb - of a split: a multiple of 64 (128 for wide
+ * tiles).  Records that point past Tq or Tk are cut there.  Bounded waits
+ * report through vcattn_attn_status as 500 + site. */
 typedef struct vcattn_packed_tile {
   int32_t q0, lq;   /* first query row in the packed buffer, queries   */
   int32_t k0, lk;   /* first key row, keys                             */
@@ -393,10 +397,17 @@ typedef struct vcattn_packed_join {
   int32_t slot0, pieces;     /* partial results [slot0, slot0 + pieces) */
   int32_t unused[3];
 } vcattn_packed_join;
-VCATTN_API size_t vcattn_attn_packed_workspace_bytes(int slots, int Hk, int D);
+typedef struct vcattn_packed_work {
+  const vcattn_packed_tile* tiles;        /* device pointers            */
+  const vcattn_packed_join* joins;
+  const vcattn_packed_tile* wide_tiles;
+  const vcattn_packed_join* wide_joins;
+  int32_t n_tiles, n_joins, slots;
+  int32_t n_wide, n_wide_joins, wide_slots;
+} vcattn_packed_work;
+VCATTN_API size_t vcattn_attn_packed_workspace_bytes(const vcattn_packed_work* work, int Hq, int Hk, int D);
 VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, const vcattn_bhnd* v, int dtype, int Hq,
-                       int Hk, int Tq, int Tk, int D, const vcattn_packed_tile* tiles, int n_tiles,
-                       const vcattn_packed_join* joins, int n_joins, int slots, int causal, float scale,
+                       int Hk, int Tq, int Tk, int D, const vcattn_packed_work* work, int causal, float scale,
                        const vcattn_bhnd* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- element codecs, exposed for bit-exact tests ------------------------

@@ -56,50 +56,56 @@ def test_rope_tables_refusals():
             rope_tables(pos, **bad)
 
 
-def _covered(plan, ql, kl):
+def _covered(tiles, joins, g, size, step, ql, kl):
     """Times each (row, key) pair of each sequence is visited, and the rows written."""
-    g = plan.heads // plan.kv_heads
     seen = [np.zeros((a * g, b), dtype=int) for a, b in zip(ql, kl)]
     rows = [np.zeros(a * g, dtype=int) for a in ql]
     q0 = np.cumsum(ql) - ql
     joined = {}
-    for j in plan.joins.numpy():
+    for j in joins.numpy():
         assert j[4] >= 2
         for s in range(j[3], j[3] + j[4]):
             assert s not in joined
             joined[s] = (j[0], j[2])
     used = set()
-    for t in plan.tiles.numpy():
+    for t in tiles.numpy():
         i = [x for x in range(len(ql)) if q0[x] == t[0] and ql[x] == t[1] and t[1] > 0][0]
-        r = slice(t[4], min(t[4] + 64, ql[i] * g))
-        assert r.start < r.stop and 0 <= t[5] <= max(t[5], t[6]) <= kl[i]
+        r = slice(t[4], min(t[4] + size, ql[i] * g))
+        assert r.start < r.stop and 0 <= t[5] <= max(t[5], t[6]) <= kl[i] and t[5] % step == 0
         seen[i][r, t[5]:t[6]] += 1
         if t[7] < 0:
             rows[i][r] += 1
         else:
-            assert joined[t[7]] == (t[0], t[4]) and t[7] not in used and t[5] % 64 == 0
+            assert joined[t[7]] == (t[0], t[4]) and t[7] not in used
             used.add(t[7])
-    assert used == set(joined) and len(used) == plan.slots
-    for j in plan.joins.numpy():
-        i = [x for x in range(len(ql)) if q0[x] == j[0] and ql[x] == j[1]][0]
-        rows[i][j[2]:min(j[2] + 64, ql[i] * g)] += 1
-    return seen, rows
+    assert used == set(joined)
+    for j in joins.numpy():
+        i = [x for x in range(len(ql)) if q0[x] == j[0] and ql[x] == j[1] and ql[x] > 0][0]
+        rows[i][j[2]:min(j[2] + size, ql[i] * g)] += 1
+    return seen, rows, len(used)
 
 
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("ql,kl,hq,hk", [
     ([1], [1], 1, 1), ([1, 1, 1], [8192, 1, 700], 8, 2), ([0, 5, 0], [3, 0, 0], 4, 4), ([200, 33], [200, 900], 4, 1),
-    ([300], [20], 5, 1), ([1000], [1000], 2, 2), ([100, 1], [5000, 129], 40, 8)])
+    ([300], [20], 5, 1), ([1000], [1000], 2, 2), ([100, 1], [5000, 129], 40, 8),
+    ([64, 63, 257, 0], [64, 2000, 4100, 7], 2, 2), ([256], [3000], 1, 1)])
 def test_plan_covers_every_pair_once(ql, kl, hq, hk, causal):
     plan = packed_plan(ql, kl, heads=hq, kv_heads=hk, head_dim=64, causal=causal, device="cpu")
     assert plan.total_q == sum(ql) and plan.total_k == sum(kl)
-    seen, rows = _covered(plan, ql, kl)
     g = hq // hk
-    for s, r, a, b in zip(seen, rows, ql, kl):
-        assert (r == 1).all() and s.max(initial=0) <= 1
-        for row in range(a * g):
-            lim = b if not causal else min(b, max(0, row // g + 1 + b - a))
-            assert (s[row, :lim] == 1).all()
+    narrow = _covered(plan.tiles, plan.joins, g, 64, 64, ql, kl)
+    wide = _covered(plan.wide_tiles, plan.wide_joins, 1, 256, 128, ql, kl)
+    assert (narrow[2], wide[2]) == (plan.work.slots, plan.work.wide_slots)
+    assert plan.workspace_bytes == N.lib().vcattn_attn_packed_workspace_bytes(plan.work, hq, hk, 64)
+    for i, (a, b) in enumerate(zip(ql, kl)):
+        took = [(s[i], r[i], grp) for (s, r, _), grp in ((narrow, g), (wide, 1)) if r[i].any()]
+        assert len(took) == (1 if a else 0)
+        for s, r, grp in took:
+            assert (r == 1).all() and s.max(initial=0) <= 1
+            for row in range(a * grp):
+                lim = b if not causal else min(b, max(0, row // grp + 1 + b - a))
+                assert (s[row, :lim] == 1).all()
 
 
 def test_plan_refusals():
@@ -154,15 +160,16 @@ def test_c_entry_points_check_their_arguments():
         assert mm(**kw) == N.ERR_ARG and text in lib.vcattn_last_error(), kw
     assert mm(m=0) == N.OK
 
-    def attn(q=None, dtype=0, hq=4, hk=2, D=64, tiles=P, slots=0, scale=0.1, ws=None, wsb=0):
-        return lib.vcattn_attn_packed(q or view(), view(), view(), dtype, hq, hk, 8, 8, D, tiles, 1, None, 0, slots, 0,
-                                      scale, view(), ws, wsb, None)
+    def attn(q=None, dtype=0, hq=4, hk=2, D=64, tiles=P, slots=0, scale=0.1, ws=None, wsb=0, n=1):
+        work = N.PackedWork(tiles, None, None, None, n, 0, slots, 0, 0, 0)
+        return lib.vcattn_attn_packed(q or view(), view(), view(), dtype, hq, hk, 8, 8, D, work, 0, scale, view(),
+                                      ws, wsb, None)
 
     for kw, text in ((dict(dtype=2), b"dtype"), (dict(hq=3), b"multiple"), (dict(D=96), b"D must"),
-                     (dict(tiles=None), b"null"), (dict(scale=-1.0), b"scale"), (dict(q=view(P + 8)), b"aligned")):
+                     (dict(tiles=None), b"null"), (dict(scale=-1.0), b"scale"), (dict(q=view(P + 8)), b"aligned"),
+                     (dict(n=-1), b"negative")):
         assert attn(**kw) == N.ERR_ARG and text in lib.vcattn_last_error(), kw
     assert attn(slots=3, ws=P, wsb=16) == N.ERR_WORKSPACE
-    assert lib.vcattn_attn_packed_workspace_bytes(3, 2, 64) >= 3 * 2 * 64 * 66 * 4
     for name, call in (("vcattn_qk_norm_rope", rope), ("vcattn_quantize_blocks", quant), ("vcattn_matmul_blocks", mm),
                        ("vcattn_attn_packed", attn)):
         N.inject_fault(name)
