@@ -39,10 +39,13 @@ struct PackedArgs {
   float* part_ml;     // [slot][head][rows][2]: reference (log2 domain) and sum
 };
 
-// Rows of a tile, and so of a partial result: (token, group head) pairs of one
-// KV head on register MMAs, tokens of one query head on tcgen05.
+// Rows of a tile, and so of a partial result, of the three lists of a batch:
+// (token, group head) pairs of one KV head on register MMAs, tokens of one
+// query head on tcgen05.
+constexpr int kPackedFewRows = 16;
 constexpr int kPackedRows = 64;
 constexpr int kPackedWideRows = 256;
+constexpr int kListRows[3] = {kPackedFewRows, kPackedRows, kPackedWideRows};
 
 cudaError_t launch_attn_packed_tc(const PackedArgs& a, int dtype, cudaStream_t st);
 

@@ -65,9 +65,8 @@ class RouteStats(Structure):
 
 class PackedWork(Structure):
     """vcattn_packed_work: the device records of a packed batch."""
-    _fields_ = [("tiles", c_void_p), ("joins", c_void_p), ("wide_tiles", c_void_p), ("wide_joins", c_void_p),
-                ("n_tiles", c_int32), ("n_joins", c_int32), ("slots", c_int32),
-                ("n_wide", c_int32), ("n_wide_joins", c_int32), ("wide_slots", c_int32)]
+    _fields_ = [("tiles", c_void_p * 3), ("joins", c_void_p * 3), ("n_tiles", c_int32 * 3), ("n_joins", c_int32 * 3),
+                ("slots", c_int32 * 3)]
 
 
 _SIGNATURES = {

@@ -14,7 +14,7 @@ register MMAs over the rows of a KV head's group for few).  Forward only.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -27,11 +27,12 @@ __all__ = ["PackedPlan", "packed_plan", "packed_attention"]
 
 SMS = 148
 
-# Rows of a tile, keys it takes at a time, and the shortest key range worth a
-# tile of its own: register-MMA tiles of (token, group head) rows, and tcgen05
-# tiles of tokens.
-NARROW = (64, 64, 256)
-WIDE = (256, 128, 1024)
+# Rows of a tile, granularity of a key range, the shortest range worth a tile of
+# its own, and the tiles per SM that keep it busy: register-MMA tiles of (token,
+# group head) rows, and tcgen05 tiles of tokens.
+FEW = (16, 64, 256, 4)
+MID = (64, 64, 256, 4)
+WIDE = (256, 128, 1024, 1)
 WIDE_FROM = 64   # queries of a sequence that goes to the tcgen05 kernel
 
 
@@ -44,16 +45,14 @@ class PackedPlan:
     causal: bool
     total_q: int
     total_k: int
-    tiles: torch.Tensor         # (n, 8) int32 records of vcattn_packed_tile
-    joins: torch.Tensor         # (n, 8) int32 records of vcattn_packed_join
-    wide_tiles: torch.Tensor
-    wide_joins: torch.Tensor
-    work: N.PackedWork          # the four arrays for the C ABI
-    workspace_bytes: int        # partial results of one call
+    tiles: Tuple[torch.Tensor, ...]   # three lists of (n, 8) int32 vcattn_packed_tile records: FEW, MID, WIDE
+    joins: Tuple[torch.Tensor, ...]   # and of vcattn_packed_join records
+    work: N.PackedWork                # the lists for the C ABI
+    workspace_bytes: int              # partial results of one call
 
     @property
     def device(self) -> torch.device:
-        return self.tiles.device
+        return self.tiles[0].device
 
 
 def _lengths(x, what) -> np.ndarray:
@@ -69,7 +68,7 @@ def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
     """Tile and join records (int32 arrays) of the given sequences, and the
     number of partial results.  A batch that would leave SMs idle splits its
     longest key ranges."""
-    rows, step, least = shape
+    rows, step, least, per_sm = shape
     per = -(-(ql * group) // rows)
     seq = np.repeat(np.arange(len(ql)), per)
     r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * rows
@@ -78,9 +77,8 @@ def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
     ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk.copy()
     pieces = np.ones(len(seq), dtype=np.int64)
     work = int(ke.sum()) * heads
-    slots = 4 * SMS if shape is NARROW else SMS
-    if len(seq) * heads < slots and work:
-        pieces = np.maximum(1, -(-ke // max(least, -(-work // slots))))
+    if len(seq) * heads < per_sm * SMS and work:
+        pieces = np.maximum(1, -(-ke // max(least, -(-work // (per_sm * SMS)))))
     span = -(-(-(-ke // pieces)) // step) * step             # keys per piece
     pieces = np.maximum(1, -(-ke // np.maximum(span, 1)))
     row = np.repeat(np.arange(len(seq)), pieces)
@@ -90,7 +88,7 @@ def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
     slot = np.where(split, np.cumsum(split) - 1, -1)
     tiles = np.stack([q0[seq][row], lq[row], k0[seq][row], lk[row], r0[row], kb,
                       np.minimum(kb + span[row], ke[row]), slot], axis=1).astype(np.int32)
-    tiles = tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")]   # longest first
+    tiles = np.ascontiguousarray(tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")])   # longest first
     js = np.nonzero(pieces > 1)[0]
     joins = np.zeros((len(js), 8), dtype=np.int32)
     joins[:, 0], joins[:, 1], joins[:, 2] = q0[seq][js], lq[js], r0[js]
@@ -123,16 +121,19 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
         raise ValueError("a sequence has 2^31 rows or more")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     q0, k0 = np.cumsum(ql) - ql, np.cumsum(kl) - kl
-    wide = ql >= WIDE_FROM
-    parts = [_tiles(q0[s], ql[s], k0[s], kl[s], *how) for s, how in
-             ((~wide, (g, kv_heads, causal, NARROW)), (wide, (1, heads, causal, WIDE)))]
-    put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
-    (tiles, joins, slots), (wtiles, wjoins, wslots) = ((put(t), put(j), s) for t, j, s in parts)
-    work = N.PackedWork(tiles.data_ptr(), joins.data_ptr(), wtiles.data_ptr(), wjoins.data_ptr(), tiles.shape[0],
-                        joins.shape[0], slots, wtiles.shape[0], wjoins.shape[0], wslots)
-    need = (slots * kv_heads * NARROW[0] + wslots * heads * WIDE[0]) * (head_dim + 2) * 4
-    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), tiles, joins, wtiles,
-                      wjoins, work, need)
+    wide, few = ql >= WIDE_FROM, ql * g <= FEW[0]
+    lists = ((few & ~wide, g, kv_heads, FEW), (~few & ~wide, g, kv_heads, MID), (wide, 1, heads, WIDE))
+    tiles, joins, slots, need = [], [], [], 0
+    for pick, group, hs, shape in lists:
+        t, j, n = _tiles(q0[pick], ql[pick], k0[pick], kl[pick], group, hs, causal, shape)
+        tiles.append(torch.from_numpy(t).to(dev))
+        joins.append(torch.from_numpy(j).to(dev))
+        slots.append(n)
+        need += n * hs * shape[0] * (head_dim + 2) * 4
+    work = N.PackedWork(tuple(t.data_ptr() for t in tiles), tuple(j.data_ptr() for j in joins),
+                        tuple(t.shape[0] for t in tiles), tuple(j.shape[0] for j in joins), tuple(slots))
+    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), tuple(tiles), tuple(joins),
+                      work, need)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,

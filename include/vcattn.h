@@ -377,14 +377,14 @@ VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float*
  * key gives 0.  P is rounded to the input type for the P V product, sums and
  * statistics are fp32.
  * Strides of k and v may not be 0 over a dimension of more than one.
- * The host lays the work out once per batch as device arrays of records.
- * `tiles` run on register MMAs: 64 rows of one KV head, row = token * Hq/Hk +
- * g; `wide_tiles` run on tcgen05: 256 rows of one query head, row = token.
- * Every query row belongs to one tile, or to the tiles of one join where its
- * keys are split over several; those write `slots` partial results that the
- * joins add up in key order.  kb - of a split: a multiple of 64 (128 for wide
- * tiles).  Records that point past Tq or Tk are cut there.  Bounded waits
- * report through vcattn_attn_status as 500 + site. */
+ * The host lays the work out once per batch as three lists of records on the
+ * device.  Lists 0 and 1 run on register MMAs: 16 and 64 rows of one KV head,
+ * row = token * Hq/Hk + g.  List 2 runs on tcgen05: 256 rows of one query
+ * head, row = token.  Every query row belongs to one tile, or to the tiles of
+ * one join where its keys are split over several; those write `slots` partial
+ * results that the joins add up in key order.  kb of a split: a multiple of 64
+ * (128 in list 2).  Records that point past Tq or Tk are cut there.  Bounded
+ * waits report through vcattn_attn_status as 500 + site. */
 typedef struct vcattn_packed_tile {
   int32_t q0, lq;   /* first query row in the packed buffer, queries   */
   int32_t k0, lk;   /* first key row, keys                             */
@@ -398,12 +398,9 @@ typedef struct vcattn_packed_join {
   int32_t unused[3];
 } vcattn_packed_join;
 typedef struct vcattn_packed_work {
-  const vcattn_packed_tile* tiles;        /* device pointers            */
-  const vcattn_packed_join* joins;
-  const vcattn_packed_tile* wide_tiles;
-  const vcattn_packed_join* wide_joins;
-  int32_t n_tiles, n_joins, slots;
-  int32_t n_wide, n_wide_joins, wide_slots;
+  const vcattn_packed_tile* tiles[3];     /* device pointers            */
+  const vcattn_packed_join* joins[3];
+  int32_t n_tiles[3], n_joins[3], slots[3];
 } vcattn_packed_work;
 VCATTN_API size_t vcattn_attn_packed_workspace_bytes(const vcattn_packed_work* work, int Hq, int Hk, int D);
 VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, const vcattn_bhnd* v, int dtype, int Hq,

@@ -94,12 +94,12 @@ def test_plan_covers_every_pair_once(ql, kl, hq, hk, causal):
     plan = packed_plan(ql, kl, heads=hq, kv_heads=hk, head_dim=64, causal=causal, device="cpu")
     assert plan.total_q == sum(ql) and plan.total_k == sum(kl)
     g = hq // hk
-    narrow = _covered(plan.tiles, plan.joins, g, 64, 64, ql, kl)
-    wide = _covered(plan.wide_tiles, plan.wide_joins, 1, 256, 128, ql, kl)
-    assert (narrow[2], wide[2]) == (plan.work.slots, plan.work.wide_slots)
+    groups, shapes = (g, g, 1), ((16, 64), (64, 64), (256, 128))
+    lists = [_covered(plan.tiles[i], plan.joins[i], groups[i], *shapes[i], ql, kl) for i in range(3)]
+    assert [x[2] for x in lists] == list(plan.work.slots)
     assert plan.workspace_bytes == N.lib().vcattn_attn_packed_workspace_bytes(plan.work, hq, hk, 64)
     for i, (a, b) in enumerate(zip(ql, kl)):
-        took = [(s[i], r[i], grp) for (s, r, _), grp in ((narrow, g), (wide, 1)) if r[i].any()]
+        took = [(s[i], r[i], grp) for (s, r, _), grp in zip(lists, groups) if r[i].any()]
         assert len(took) == (1 if a else 0)
         for s, r, grp in took:
             assert (r == 1).all() and s.max(initial=0) <= 1
@@ -161,7 +161,7 @@ def test_c_entry_points_check_their_arguments():
     assert mm(m=0) == N.OK
 
     def attn(q=None, dtype=0, hq=4, hk=2, D=64, tiles=P, slots=0, scale=0.1, ws=None, wsb=0, n=1):
-        work = N.PackedWork(tiles, None, None, None, n, 0, slots, 0, 0, 0)
+        work = N.PackedWork((None, tiles, None), (None,) * 3, (0, n, 0), (0, 0, 0), (0, slots, 0))
         return lib.vcattn_attn_packed(q or view(), view(), view(), dtype, hq, hk, 8, 8, D, work, 0, scale, view(),
                                       ws, wsb, None)
 
