@@ -10,56 +10,63 @@ import torch
 
 from . import _native as N
 
+DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16, torch.float32: N.DTYPE_F32}
+
 _SAME_DEVICE = nullcontext()
+# The current device and raw stream without building Python objects for them
+# (a call's host time is what a small launch costs); the public calls where a
+# torch build lacks these.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def refuse_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """The operators have no backward pass: say so instead of cutting the graph."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def on_device(device: torch.device):
     """Context in which ``device`` is current (nothing to do when it already is)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME_DEVICE if _current_device() == device.index else torch.cuda.device(device)
 
 
 def stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def rows_aligned(x: torch.Tensor) -> bool:
-    """(B, H, N, D) with contiguous channels and every row on a 16-byte boundary."""
-    sb, sh, sn, sd = x.stride()
-    return sd == 1 and (x.data_ptr() | sb * x.element_size() | sh * x.element_size() | sn * x.element_size()) & 15 == 0
+    """The current stream of ``device``."""
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def view(x: torch.Tensor) -> Tuple[N.BHND, torch.Tensor]:
-    """vcattn_bhnd of x and the tensor it points into (a copy if the rows are
-    not aligned, or are the same memory as those of a broadcast view)."""
-    if not rows_aligned(x) or (0 in x.stride() and x.numel() > x.shape[-1]):
+    """vcattn_bhnd of a (B, H, N, D) tensor and the tensor it points into: a
+    copy if the channels are not contiguous, a row is not on a 16-byte boundary
+    or rows are the same memory (a broadcast view)."""
+    sb, sh, sn, sd = x.stride()
+    p = x.data_ptr()
+    if sd != 1 or (p | (sb | sh | sn) * x.element_size()) & 15 or not (sb and sh and sn):
         x = x.clone(memory_format=torch.contiguous_format)
-    sb, sh, sn, _ = x.stride()
-    return N.BHND(x.data_ptr(), sb, sh, sn), x
+        sb, sh, sn, _ = x.stride()
+        p = x.data_ptr()
+    return N.BHND(p, sb, sh, sn), x
 
 
-def empty_like_rows(x: torch.Tensor) -> torch.Tensor:
-    """Output buffer in the token layout of a (B, H, N, D) input: token-major
-    rows (the ComfyUI (B, N, H*D) path) stay token-major."""
-    b, h, n, d = x.shape
-    if x.stride(1) < x.stride(2):
-        return torch.empty((b, n, h, d), dtype=x.dtype, device=x.device).transpose(1, 2)
-    return torch.empty((b, h, n, d), dtype=x.dtype, device=x.device)
-
-
-def out_rows(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> torch.Tensor:
-    """``out`` checked against its input, or a new buffer."""
+def out_view(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> Tuple[N.BHND, torch.Tensor]:
+    """``out`` checked against its input, or a new buffer in the token layout of
+    the input: token-major rows (the ComfyUI (B, N, H*D) path) stay so."""
     if out is None:
-        return empty_like_rows(x)
+        b, h, n, d = x.shape
+        if x.stride(1) < x.stride(2):
+            out = torch.empty_strided((b, h, n, d), (n * h * d, d, h * d, 1), dtype=x.dtype, device=x.device)
+        else:
+            out = torch.empty((b, h, n, d), dtype=x.dtype, device=x.device)
+        sb, sh, sn, _ = out.stride()
+        if (sb | sh | sn) * x.element_size() & 15:   # rows of an odd length
+            raise ValueError(f"rows of {d} channels of {x.dtype} do not start on 16-byte boundaries")
+        return N.BHND(out.data_ptr(), sb, sh, sn), out
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{what} must match its input: {tuple(x.shape)} {x.dtype} on {x.device}")
-    if out.numel() and (not rows_aligned(out) or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape))):
+    sb, sh, sn, sd = out.stride()
+    if out.numel() and (sd != 1 or (out.data_ptr() | (sb | sh | sn) * out.element_size()) & 15
+                        or any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape))):
         raise ValueError(f"{what} must have contiguous channels and 16-byte aligned rows of their own")
-    return out
+    return N.BHND(out.data_ptr(), sb, sh, sn), out

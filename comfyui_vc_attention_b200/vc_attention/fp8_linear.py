@@ -17,8 +17,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from ._launch import on_device, refuse_grad, stream
-from .grouping import _dtype_code
+from ._launch import DTYPES, on_device, refuse_grad, stream
 
 __all__ = ["Fp8Blocks", "quantize_blocks", "matmul_blocks", "linear_blocks"]
 
@@ -41,50 +40,52 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Fp8Blocks:
     E4M3(x / scale), round to nearest even.  The scales are stored with rows
     side by side (the order the product reads them in).
     """
-    refuse_grad("quantize_blocks", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        refuse_grad("quantize_blocks", x)
     if not x.is_cuda:
         raise RuntimeError("quantize_blocks needs a CUDA tensor (this build has no CPU path)")
     if rows not in (1, BLOCK):
         raise ValueError(f"rows must be 1 or {BLOCK}, got {rows}")
-    dt = _dtype_code(x)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x must be (M, K) with K > 0, got {tuple(x.shape)}")
-    k = x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    xs = x.shape
+    if len(xs) < 1 or xs[-1] == 0:
+        raise ValueError(f"x must be (M, K) with K > 0, got {tuple(xs)}")
+    k = xs[-1]
+    x2 = x if len(xs) == 2 else x.reshape(-1, k)
     m = x2.shape[0]
-    if x2.stride(1) != 1 or (m > 1 and x2.stride(0) < k):
-        x2 = x2.contiguous()
-    ldx = x2.stride(0) if m > 1 else k
+    ldx, sk = x2.stride()
+    if (sk != 1 and k > 1) or (m > 1 and ldx < k):
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+        ldx = k
+    dev = x.device
     ldc = -(-k // 16) * 16
-    codes = torch.empty((m, ldc), dtype=torch.float8_e4m3fn, device=x.device)
-    if ldc != k:
-        codes = codes[:, :k]
-    kb = -(-k // BLOCK)
-    scale = torch.empty((kb, -(-m // rows)), dtype=torch.float32, device=x.device)
-    with on_device(x.device):
+    codes = torch.empty((m, ldc), dtype=torch.float8_e4m3fn, device=dev)
+    mb = m if rows == 1 else -(-m // rows)
+    scale = torch.empty_strided((mb, -(-k // BLOCK)), (1, mb), dtype=torch.float32, device=dev)
+    with on_device(dev):
         N.check("vcattn_quantize_blocks", N.lib().vcattn_quantize_blocks(
-            x2.data_ptr(), dt, m, k, ldx, rows, codes.data_ptr(), ldc, scale.data_ptr(), 1, scale.shape[1], stream(x.device)))
-    return Fp8Blocks(codes, scale.t(), rows)
+            x2.data_ptr(), dt, m, k, max(ldx, k), rows, codes.data_ptr(), ldc, scale.data_ptr(), 1, mb, stream(dev)))
+    return Fp8Blocks(codes if ldc == k else codes[:, :k], scale, rows)
 
 
-def _check_blocks(b: Fp8Blocks, name: str, rows: int):
-    if not (b.codes.is_cuda and b.scale.is_cuda) or b.codes.device != b.scale.device:
+def _code_rows(b: Fp8Blocks, name: str, rows: int):
+    """(codes, row pitch) of a checked operand as the TMA reads them: 16-byte rows, copied if need be."""
+    c, s = b.codes, b.scale
+    if not (c.is_cuda and s.is_cuda) or c.device != s.device:
         raise RuntimeError(f"matmul_blocks needs CUDA tensors on one device ({name})")
     if b.rows != rows:
         raise ValueError(f"{name} must have one scale per {rows} row(s) and {BLOCK} columns, got rows={b.rows}")
-    if b.codes.dtype != torch.float8_e4m3fn or b.codes.dim() != 2 or b.codes.shape[1] == 0:
-        raise ValueError(f"{name}.codes must be (rows, K) float8_e4m3fn, got {tuple(b.codes.shape)} {b.codes.dtype}")
-    m, k = b.codes.shape
-    want = (-(-m // rows), -(-k // BLOCK))
-    if b.scale.dtype != torch.float32 or tuple(b.scale.shape) != want:
-        raise ValueError(f"{name}.scale must be {want} float32, got {tuple(b.scale.shape)} {b.scale.dtype}")
-
-
-def _code_rows(c: torch.Tensor):
-    """(tensor, row pitch): codes as the TMA reads them (16-byte rows), copied if need be."""
+    if c.dtype != torch.float8_e4m3fn or c.dim() != 2 or c.shape[1] == 0:
+        raise ValueError(f"{name}.codes must be (rows, K) float8_e4m3fn, got {tuple(c.shape)} {c.dtype}")
     m, k = c.shape
-    ld = c.stride(0) if m > 1 else -(-k // 16) * 16
-    if c.stride(1) == 1 and c.data_ptr() % 16 == 0 and ld % 16 == 0 and ld >= k:
+    if s.dtype != torch.float32 or s.shape != (-(-m // rows), -(-k // BLOCK)):
+        raise ValueError(f"{name}.scale must be {(-(-m // rows), -(-k // BLOCK))} float32, got {tuple(s.shape)} {s.dtype}")
+    ld, sk = c.stride()
+    if m <= 1:
+        ld = -(-k // 16) * 16   # (the pitch of a single row is never used)
+    if (sk == 1 or k == 1) and (c.data_ptr() | ld) & 15 == 0 and ld >= k:
         return c, ld
     ld = -(-k // 16) * 16
     t = torch.empty((m, ld), dtype=c.dtype, device=c.device)
@@ -101,33 +102,39 @@ def matmul_blocks(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = Non
     is rounded once.  bias: (N,) or None.  out: (M, N) of ``dtype`` with
     contiguous columns, or None.
     """
-    _check_blocks(a, "a", 1)
-    _check_blocks(b, "b", BLOCK)
-    refuse_grad("matmul_blocks", a.scale, b.scale, bias)
+    if torch.is_grad_enabled():
+        refuse_grad("matmul_blocks", a.scale, b.scale, bias)
+    ac, lda = _code_rows(a, "a", 1)
+    bc, ldb = _code_rows(b, "b", BLOCK)
     m, k = a.codes.shape
-    n = b.codes.shape[0]
-    dev = a.codes.device
-    if b.codes.shape[1] != k or b.codes.device != dev:
+    n, kb = b.codes.shape
+    dev = ac.device
+    if kb != k or bc.device != dev:
         raise ValueError(f"a and b must share K and a device, got {tuple(a.codes.shape)} on {dev}, "
-                         f"{tuple(b.codes.shape)} on {b.codes.device}")
+                         f"{tuple(b.codes.shape)} on {bc.device}")
+    bp = None
     if bias is not None:
         if bias.shape != (n,) or bias.device != dev:
             raise ValueError(f"bias must be ({n},) on {dev}, got {tuple(bias.shape)} on {bias.device}")
-        bias = bias.to(torch.float32).contiguous()
+        if bias.dtype != torch.float32 or bias.stride(0) != 1:
+            bias = bias.to(torch.float32).contiguous()
+        bp = bias.data_ptr()
+    odt = DTYPES.get(dtype)
+    if odt is None:
+        raise TypeError(f"unsupported dtype {dtype}")
     if out is None:
         out = torch.empty((m, n), dtype=dtype, device=dev)
-    elif out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or \
-            (m > 1 and out.stride(0) < n):
-        raise ValueError(f"out must be ({m}, {n}) {dtype} on {dev} with contiguous columns")
-    odt = _dtype_code(out)
-    ac, lda = _code_rows(a.codes)
-    bc, ldb = _code_rows(b.codes)
-    ldo = out.stride(0) if m > 1 else max(n, 1)
+        ldo = max(n, 1)
+    else:
+        if out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or \
+                (m > 1 and out.stride(0) < n):
+            raise ValueError(f"out must be ({m}, {n}) {dtype} on {dev} with contiguous columns")
+        ldo = out.stride(0) if m > 1 else max(n, 1)
+    (sam, sak), (sbn, sbk) = a.scale.stride(), b.scale.stride()
     with on_device(dev):
         N.check("vcattn_matmul_blocks", N.lib().vcattn_matmul_blocks(
-            ac.data_ptr(), lda, a.scale.data_ptr(), a.scale.stride(0), a.scale.stride(1),
-            bc.data_ptr(), ldb, b.scale.data_ptr(), b.scale.stride(0), b.scale.stride(1), m, n, k,
-            None if bias is None else bias.data_ptr(), out.data_ptr(), odt, ldo, stream(dev)))
+            ac.data_ptr(), lda, a.scale.data_ptr(), sam, sak, bc.data_ptr(), ldb, b.scale.data_ptr(), sbn, sbk, m, n, k,
+            bp, out.data_ptr(), odt, ldo, stream(dev)))
     return out
 
 

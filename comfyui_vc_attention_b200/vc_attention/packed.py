@@ -20,8 +20,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from ._launch import on_device, out_rows, refuse_grad, stream, view
-from .grouping import _dtype_code
+from ._launch import DTYPES, on_device, out_view, refuse_grad, stream, view
 
 __all__ = ["PackedPlan", "packed_plan", "packed_attention"]
 
@@ -146,7 +145,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     writes ``out``.  Scores, statistics and sums are fp32; P is rounded to q's
     type for the second product.
     """
-    refuse_grad("packed_attention", q, k, v)
+    if torch.is_grad_enabled():
+        refuse_grad("packed_attention", q, k, v)
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("packed_attention needs CUDA tensors (this build has no CPU path)")
     d = plan.head_dim
@@ -154,21 +154,21 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     if q.shape != want_q or k.shape != want_k or v.shape != want_k:
         raise ValueError(f"the plan needs q {want_q} and k, v {want_k}, got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype, dev = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"q, k, v must share bfloat16 or float16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if not q.device == k.device == v.device == plan.device:
+    if not dev == k.device == v.device == plan.device:
         raise ValueError("q, k, v and the plan must be on one device")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    out = out_rows(out, q, "out")
-    if plan.total_q == 0:
-        return out
-    (qv, q), (kv, k), (vv, v), (ov, _) = view(q), view(k), view(v), view(out)
-    ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device) if plan.workspace_bytes else None
-    with on_device(q.device):
+    ov, out = out_view(out, q, "out")
+    (qv, q), (kv, k), (vv, v) = view(q), view(k), view(v)   # (what a view points into lives until the launch)
+    need, ws = plan.workspace_bytes, None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with on_device(dev):
         N.check("vcattn_attn_packed", N.lib().vcattn_attn_packed(
-            qv, kv, vv, _dtype_code(q), plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d, plan.work,
-            int(plan.causal), scale, ov, None if ws is None else ws.data_ptr(), plan.workspace_bytes,
-            stream(q.device)))
+            qv, kv, vv, DTYPES[dtype], plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d, plan.work, plan.causal,
+            scale, ov, None if ws is None else ws.data_ptr(), need, stream(dev)))
     return out
