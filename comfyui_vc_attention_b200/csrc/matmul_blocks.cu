@@ -5,8 +5,11 @@
 // tcgen05 kind::f8f6f4: each k-block of 128 is one accumulation of four MMAs in
 // tensor memory, in one of two buffers; the promotion warps read the finished
 // block sum and add it to fp32 registers with its scale while the next block
-// runs.  Thread = output row (TMEM lane), so the scale of a block is one
-// scalar per thread and 128 columns.
+// runs.  Thread = output row (TMEM lane) and 64 columns, so the scale of a
+// block is one scalar per thread.
+//   warp 0       TMA producer        warp 1   MMA issuer, tensor-memory owner
+//   warps 2-3    sa * sb of each k-block into a ring in shared memory
+//   warps 4-     promotion and output
 #include <cuda.h>
 #include <mutex>
 #include <string>
@@ -37,20 +40,29 @@ struct MatmulArgs {
   int vec_out;   // rows of `out` start on 16-byte boundaries
 };
 
+constexpr int kScales = 8;   // k-blocks that the scale ring holds
+
 template <int BN> struct MmCfg {
-  static constexpr int kStages = BN == 256 ? 4 : 6;
-  static constexpr int kPromo = BN / 128;                  // promotion warpgroups
-  static constexpr int kThreads = 128 + 128 * kPromo;
+  static constexpr int kStages = BN == 256 ? 3 : 5;
+  static constexpr int kPromo = BN / 64 * 4;               // promotion warps
+  static constexpr int kThreads = 128 + 32 * kPromo;
   static constexpr int kTmemCols = 2 * BN;
+  // Output staging of a warp: 32 rows of 64 16-bit values (or 32 fp32 values),
+  // 16 bytes apart more than their length so that the rows start in different banks.
+  static constexpr int kOutPitch = 128 + 16;
 };
 
 template <int BN> struct MmSmem {
   alignas(1024) uint8_t a[MmCfg<BN>::kStages][kBM * kBK];
   alignas(1024) uint8_t b[MmCfg<BN>::kStages][BN * kBK];
+  alignas(16) uint8_t out[MmCfg<BN>::kPromo][32 * MmCfg<BN>::kOutPitch];
+  alignas(16) float scale[kScales][BN / 128][kBM];
   alignas(8) uint64_t full[MmCfg<BN>::kStages];
   alignas(8) uint64_t empty[MmCfg<BN>::kStages];
   alignas(8) uint64_t t_full[2];
   alignas(8) uint64_t t_empty[2];
+  alignas(8) uint64_t s_full[kScales];
+  alignas(8) uint64_t s_empty[kScales];
   alignas(8) uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -85,7 +97,11 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.t_full[b], 1);
-      mbar_init(&sm.t_empty[b], 4 * Cfg::kPromo);
+      mbar_init(&sm.t_empty[b], Cfg::kPromo);
+    }
+    for (int r = 0; r < kScales; ++r) {
+      mbar_init(&sm.s_full[r], 2);
+      mbar_init(&sm.s_empty[r], Cfg::kPromo);
     }
     mbar_init(&sm.drain, 1);
     fence_mbar_init();
@@ -98,10 +114,9 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   tc_fence_after();
   const uint32_t tbase = sm.tmem_base;
   volatile int* abort = &sm.abort;
-  // BN = 256 is launched at 168 x 384 = 64512 registers: 128 x 40 + 256 x 232
-
   if (warp < 4) {
-  if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n" ::: "memory");
+  // BN = 256 is launched at 96 x 640 = 61440 registers: 128 x 56 + 512 x 104 = 60416
+  if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n" ::: "memory");
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -156,76 +171,124 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     while (!mbar_try_wait(&sm.drain, 0) && clock64() - t0 < kWaitCycles) {
     }
     __syncwarp();
-  }
   } else {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n" ::: "memory");
-    // ------------------------------------------------------------ promotion and output
-    const int wq = warp & 3, col_half = (warp - 4) >> 2;
-    const uint32_t lb = tbase + (static_cast<uint32_t>(wq * 32) << 16) + col_half * 128;
-    constexpr int ES = ODT == VCATTN_DTYPE_F32 ? 4 : 2;
+    // ------------------------------------------------------------ scales
+    const int r = tid - 64;   // rows r and r + 64
     int it = 0;
     bool ok = true;
     for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
       int mt, nt;
       tile_coords(a, t, mt, nt);
-      const int m = mt * kBM + wq * 32 + lane;
-      const int n0 = nt * BN + col_half * 128;
-      const bool live = m < a.M && n0 < a.N;
-      const float* sa = a.sa + static_cast<int64_t>(live ? m : 0) * a.sam;
-      const float* sb = a.sb + static_cast<int64_t>(live ? n0 / 128 : 0) * a.sbn;
-      float acc[128];
+      // (rows and columns past the matrix take the scale of the last one: nothing of them is written)
+      const float* sa0 = a.sa + static_cast<int64_t>(min(mt * kBM + r, a.M - 1)) * a.sam;
+      const float* sa1 = a.sa + static_cast<int64_t>(min(mt * kBM + r + 64, a.M - 1)) * a.sam;
+      const float* sb[BN / 128];
 #pragma unroll
-      for (int c = 0; c < 128; ++c) acc[c] = 0.f;
-      float s_next = __ldg(sa) * __ldg(sb);
+      for (int c = 0; c < BN / 128; ++c) sb[c] = a.sb + static_cast<int64_t>(min(nt * BN + c * 128, a.N - 1) / 128) * a.sbn;
+      for (int k0 = 0; ok && k0 < a.kb; k0 += 4) {
+        // four blocks' scales in flight
+        float x0[4], x1[4], y[4][BN / 128];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int k = min(k0 + u, a.kb - 1);
+          x0[u] = __ldg(sa0 + k * a.sak);
+          x1[u] = __ldg(sa1 + k * a.sak);
+#pragma unroll
+          for (int c = 0; c < BN / 128; ++c) y[u][c] = __ldg(sb[c] + k * a.sbk);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (ok && k0 + u < a.kb) {
+            const int s = it % kScales;
+            if (it >= kScales) ok = mbar_wait(&sm.s_empty[s], ((it / kScales) + 1) & 1, abort, status, 5);
+#pragma unroll
+            for (int c = 0; c < BN / 128; ++c) {
+              sm.scale[s][c][r] = x0[u] * y[u][c];
+              sm.scale[s][c][r + 64] = x1[u] * y[u][c];
+            }
+            warp_arrive(&sm.s_full[s], lane);
+            ++it;
+          }
+        }
+      }
+    }
+  }
+  } else {
+    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::: "memory");
+    // ------------------------------------------------------------ promotion and output
+    const int wq = warp & 3, quarter = (warp - 4) >> 2;   // 32 rows x 64 columns
+    const uint32_t lb = tbase + (static_cast<uint32_t>(wq * 32) << 16) + quarter * 64;
+    constexpr int ES = ODT == VCATTN_DTYPE_F32 ? 4 : 2;
+    uint8_t* stage = sm.out[warp - 4];
+    int it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+      int mt, nt;
+      tile_coords(a, t, mt, nt);
+      const int m0 = mt * kBM + wq * 32, n0 = nt * BN + quarter * 64;
+      float acc[64];
+#pragma unroll
+      for (int c = 0; c < 64; ++c) acc[c] = 0.f;
       for (int k = 0; k < a.kb; ++k, ++it) {
-        const int b = it & 1;
-        const float s = s_next;
-        if (k + 1 < a.kb) s_next = __ldg(sa + (k + 1) * a.sak) * __ldg(sb + (k + 1) * a.sbk);
-        if (!(ok = mbar_wait(&sm.t_full[b], (it >> 1) & 1, abort, status, 4))) break;
+        const int b = it & 1, r = it % kScales;
+        if (!(ok = mbar_wait2(&sm.s_full[r], (it / kScales) & 1, &sm.t_full[b], (it >> 1) & 1, abort, status, 4))) break;
+        const float s = sm.scale[r][quarter >> 1][wq * 32 + lane];
         tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
+        for (int h = 0; h < 2; ++h) {
           float x[32];
           tmem_ld32(lb + b * BN + h * 32, x);
           tmem_ld_wait();
           reg_fence(x);
-          if (h == 3) {
+          if (h == 1) {
             tc_fence_before();
-            warp_arrive(&sm.t_empty[b], lane);
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&sm.t_empty[b]);
+              mbar_arrive(&sm.s_empty[r]);
+            }
           }
 #pragma unroll
           for (int c = 0; c < 32; c += 2) fma2(acc[h * 32 + c], acc[h * 32 + c + 1], x[c], x[c + 1], s, s);
         }
       }
-      if (!ok || *abort || !live) continue;
-      const int cols = min(128, a.N - n0);
-      uint8_t* o = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(m) * a.ldo + n0) * ES;
+      if (!ok || *abort) continue;
+      // rows through shared memory, so that whole 128-byte lines go out
+      constexpr int PC = 128 / ES;   // columns per pass
 #pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += 16 / ES) {
-        if (a.bias != nullptr) {
+      for (int p = 0; p < 64 / PC; ++p) {
+        const int np = n0 + p * PC;
 #pragma unroll
-          for (int e = 0; e < 16 / ES; ++e)
-            if (c0 + e < cols) acc[c0 + e] += __ldg(a.bias + n0 + c0 + e);
-        }
-        if (a.vec_out && c0 + 16 / ES <= cols) {
+        for (int c = 0; c < PC; c += 16 / ES) {
           uint4 w;
 #pragma unroll
-          for (int e = 0; e < 16 / ES; e += 2)
-            stage2<ODT>(reinterpret_cast<uint8_t*>(&w) + e * ES, acc[c0 + e], acc[c0 + e + 1]);
-          *reinterpret_cast<uint4*>(o + c0 * ES) = w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16 / ES; ++e) {
-            if (c0 + e < cols) {
-              if constexpr (ODT == VCATTN_DTYPE_BF16)
-                reinterpret_cast<__nv_bfloat16*>(o)[c0 + e] = __float2bfloat16_rn(acc[c0 + e]);
-              else if constexpr (ODT == VCATTN_DTYPE_F16)
-                reinterpret_cast<__half*>(o)[c0 + e] = __float2half_rn(acc[c0 + e]);
-              else
-                reinterpret_cast<float*>(o)[c0 + e] = acc[c0 + e];
+          for (int e = 0; e < 16 / ES; e += 2) {
+            float v0 = acc[p * PC + c + e], v1 = acc[p * PC + c + e + 1];
+            if (a.bias != nullptr) {
+              v0 += np + c + e < a.N ? __ldg(a.bias + np + c + e) : 0.f;
+              v1 += np + c + e + 1 < a.N ? __ldg(a.bias + np + c + e + 1) : 0.f;
+            }
+            stage2<ODT>(reinterpret_cast<uint8_t*>(&w) + e * ES, v0, v1);
+          }
+          *reinterpret_cast<uint4*>(stage + lane * Cfg::kOutPitch + c * ES) = w;
+        }
+        __syncwarp();
+        const int cols = min(PC, a.N - np);
+        for (int i = lane; i < 32 * 8; i += 32) {
+          const int r = i >> 3, c = (i & 7) * (16 / ES);   // 16-byte chunk of a row
+          if (m0 + r >= a.M || c >= cols) continue;
+          const uint8_t* src = stage + r * Cfg::kOutPitch + c * ES;
+          uint8_t* dst = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(m0 + r) * a.ldo + np + c) * ES;
+          if (a.vec_out && c + 16 / ES <= cols) {
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+          } else {
+            for (int e = 0; e < 16 / ES && c + e < cols; ++e) {
+              if constexpr (ES == 2) reinterpret_cast<uint16_t*>(dst)[e] = reinterpret_cast<const uint16_t*>(src)[e];
+              else reinterpret_cast<uint32_t*>(dst)[e] = reinterpret_cast<const uint32_t*>(src)[e];
             }
           }
         }
+        __syncwarp();
       }
     }
   }
