@@ -38,7 +38,44 @@ struct MatmulArgs {
   int M, N, kb;
   int mt, nt, tiles, group;
   int vec_out;   // rows of `out` start on 16-byte boundaries
+  int ranks;     // CTAs of a cluster that share a tile's k-blocks (1: persistent CTAs over whole tiles)
 };
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(const float* p, uint32_t rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+template <int ODT> __device__ __forceinline__ void store1(void* out, int64_t i, float v) {
+  if constexpr (ODT == VCATTN_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else if constexpr (ODT == VCATTN_DTYPE_F16) static_cast<__half*>(out)[i] = __float2half_rn(v);
+  else static_cast<float*>(out)[i] = v;
+}
 
 constexpr int kScales = 8;   // k-blocks that the scale ring holds
 
@@ -50,6 +87,8 @@ template <int BN> struct MmCfg {
   // Output staging of a warp: 32 rows of 64 16-bit values (or 32 fp32 values),
   // 16 bytes apart more than their length so that the rows start in different banks.
   static constexpr int kOutPitch = 128 + 16;
+  static constexpr int kPartPitch = BN + 4;   // floats of a row of a rank's sums
+  static_assert(kBM * kPartPitch * 4 <= kStages * kBM * kBK + kStages * BN * kBK, "a rank's sums fit over the stages");
 };
 
 template <int BN> struct MmSmem {
@@ -78,7 +117,7 @@ __device__ __forceinline__ void tile_coords(const MatmulArgs& a, int t, int& m, 
   m = g * a.group + (r - n * rows);
 }
 
-template <int BN, int ODT>
+template <int BN, int ODT, bool SPLIT>
 __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     matmul_blocks_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const MatmulArgs a) {
@@ -114,6 +153,11 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   tc_fence_after();
   const uint32_t tbase = sm.tmem_base;
   volatile int* abort = &sm.abort;
+  // tiles of this CTA, and the k-blocks that it takes of each
+  const int t0 = SPLIT ? blockIdx.x / a.ranks : blockIdx.x, t_step = SPLIT ? a.tiles : gridDim.x;
+  const int rank = SPLIT ? static_cast<int>(cluster_rank()) : 0;
+  const int kb0 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kb) * rank / a.ranks) : 0;
+  const int kb1 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kb) * (rank + 1) / a.ranks) : a.kb;
   if (warp < 4) {
   // BN = 256 is launched at 96 x 640 = 61440 registers: 128 x 56 + 512 x 104 = 60416
   if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n" ::: "memory");
@@ -124,10 +168,10 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       prefetch_tmap(&tm_b);
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+      for (int t = t0; ok && t < a.tiles; t += t_step) {
         int m, n;
         tile_coords(a, t, m, n);
-        for (int k = 0; k < a.kb; ++k, ++it) {
+        for (int k = kb0; k < kb1; ++k, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !(ok = mbar_wait(&sm.empty[s], ((it / kStages) + 1) & 1, abort, status, 1))) break;
           mbar_expect_tx(&sm.full[s], (kBM + BN) * kBK);
@@ -138,8 +182,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       // on an abandoned run, let the copies already issued land
       if (!ok || *abort) {
         for (int j = max(0, it - kStages); j < it; ++j) {
-          const long long t0 = clock64();
-          while (!mbar_try_wait(&sm.full[j % kStages], (j / kStages) & 1) && clock64() - t0 < kWaitCycles / 4) {
+          const long long c0 = clock64();
+          while (!mbar_try_wait(&sm.full[j % kStages], (j / kStages) & 1) && clock64() - c0 < kWaitCycles / 4) {
           }
         }
       }
@@ -151,8 +195,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const uint32_t idesc = idesc_e4m3(kBM, BN, false);
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
-      for (int k = 0; k < a.kb; ++k, ++it) {
+    for (int t = t0; ok && t < a.tiles; t += t_step) {
+      for (int k = kb0; k < kb1; ++k, ++it) {
         const int s = it % kStages, b = it & 1;
         if (it >= 2 && !(ok = mbar_wait(&sm.t_empty[b], ((it >> 1) + 1) & 1, abort, status, 2))) break;
         if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, abort, status, 3))) break;
@@ -167,8 +211,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     }
     // every MMA issued must finish before tensor memory is released
     tc_commit_if(&sm.drain, leader);
-    const long long t0 = clock64();
-    while (!mbar_try_wait(&sm.drain, 0) && clock64() - t0 < kWaitCycles) {
+    const long long c0 = clock64();
+    while (!mbar_try_wait(&sm.drain, 0) && clock64() - c0 < kWaitCycles) {
     }
     __syncwarp();
   } else {
@@ -176,7 +220,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const int r = tid - 64;   // rows r and r + 64
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+    for (int t = t0; ok && t < a.tiles; t += t_step) {
       int mt, nt;
       tile_coords(a, t, mt, nt);
       // (rows and columns past the matrix take the scale of the last one: nothing of them is written)
@@ -185,12 +229,12 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       const float* sb[BN / 128];
 #pragma unroll
       for (int c = 0; c < BN / 128; ++c) sb[c] = a.sb + static_cast<int64_t>(min(nt * BN + c * 128, a.N - 1) / 128) * a.sbn;
-      for (int k0 = 0; ok && k0 < a.kb; k0 += 4) {
+      for (int k0 = kb0; ok && k0 < kb1; k0 += 4) {
         // four blocks' scales in flight
         float x0[4], x1[4], y[4][BN / 128];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int k = min(k0 + u, a.kb - 1);
+          const int k = min(k0 + u, kb1 - 1);
           x0[u] = __ldg(sa0 + k * a.sak);
           x1[u] = __ldg(sa1 + k * a.sak);
 #pragma unroll
@@ -198,7 +242,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          if (ok && k0 + u < a.kb) {
+          if (ok && k0 + u < kb1) {
             const int s = it % kScales;
             if (it >= kScales) ok = mbar_wait(&sm.s_empty[s], ((it / kScales) + 1) & 1, abort, status, 5);
 #pragma unroll
@@ -222,14 +266,14 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     uint8_t* stage = sm.out[warp - 4];
     int it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < a.tiles; t += gridDim.x) {
+    for (int t = t0; ok && t < a.tiles; t += t_step) {
       int mt, nt;
       tile_coords(a, t, mt, nt);
       const int m0 = mt * kBM + wq * 32, n0 = nt * BN + quarter * 64;
       float acc[64];
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-      for (int k = 0; k < a.kb; ++k, ++it) {
+      for (int k = kb0; k < kb1; ++k, ++it) {
         const int b = it & 1, r = it % kScales;
         if (!(ok = mbar_wait2(&sm.s_full[r], (it / kScales) & 1, &sm.t_full[b], (it >> 1) & 1, abort, status, 4))) break;
         const float s = sm.scale[r][quarter >> 1][wq * 32 + lane];
@@ -253,6 +297,13 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         }
       }
       if (!ok || *abort) continue;
+      if constexpr (SPLIT) {
+        // this rank's sums over the operand stages (every MMA has read them)
+        float* part = reinterpret_cast<float*>(sm.a) + (wq * 32 + lane) * Cfg::kPartPitch + quarter * 64;
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) *reinterpret_cast<float4*>(part + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        continue;
+      }
       // rows through shared memory, so that whole 128-byte lines go out
       constexpr int PC = 128 / ES;   // columns per pass
 #pragma unroll
@@ -294,6 +345,212 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   }
   __syncthreads();
   if (warp == 1) tmem_dealloc(tbase, Cfg::kTmemCols);
+  if constexpr (SPLIT) {
+    // every rank adds the parts of its share of the rows, in rank order
+    __syncwarp();
+    cluster_sync();
+    int mt, nt;
+    tile_coords(a, t0, mt, nt);
+    const int rows = *abort ? 0 : min(kBM, a.M - mt * kBM);
+    for (int r = rank * (Cfg::kThreads / 32) + warp; r < rows; r += a.ranks * (Cfg::kThreads / 32)) {
+      for (int c = lane * 4; c < BN; c += 128) {
+        const int n = nt * BN + c;
+        if (n >= a.N) continue;
+        const float* p = reinterpret_cast<const float*>(sm.a) + r * Cfg::kPartPitch + c;
+        float4 v = ld_cluster4(p, 0);
+        for (int q = 1; q < a.ranks; ++q) {
+          const float4 w = ld_cluster4(p, q);
+          v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+        }
+        const float e[4] = {v.x, v.y, v.z, v.w};
+        const int64_t o = static_cast<int64_t>(mt * kBM + r) * a.ldo + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < a.N) store1<ODT>(a.out, o + i, e[i] + (a.bias != nullptr ? __ldg(a.bias + n + i) : 0.f));
+      }
+    }
+    __syncwarp();
+    cluster_sync();   // no CTA leaves while another reads its part
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------
+// For M up to 64 the weight's bytes bound the product.  Here the weight rows
+// are the MMA's 128 rows and the activations its MN columns, and the k-blocks
+// of a row tile are dealt to the CTAs of a cluster, so that every SM streams
+// weights; the partial sums meet in shared memory of the cluster and are added
+// in rank order.
+//   warp 0  TMA producer     warp 1  MMA issuer     warps 4-7  promotion, output
+constexpr int kFewStages = 4;
+
+struct FewArgs {
+  const float *sa, *sb;
+  int64_t sam, sak, sbn, sbk;
+  const float* bias;
+  void* out;
+  int64_t ldo;
+  int M, N, kb;
+};
+
+template <int MN> struct FewSmem {
+  alignas(1024) uint8_t w[kFewStages][128 * kBK];   // at the end: this CTA's sums, [activation row][weight row] fp32
+  alignas(1024) uint8_t x[kFewStages][MN * kBK];
+  alignas(16) float scale[2][MN];             // sa * sb of a k-block
+  alignas(8) uint64_t full[kFewStages];
+  alignas(8) uint64_t empty[kFewStages];
+  alignas(8) uint64_t t_full[2];
+  alignas(8) uint64_t t_empty[2];
+  alignas(8) uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <int MN, int ODT>
+__global__ void __launch_bounds__(256, MN == 16 ? 3 : 2)
+    matmul_blocks_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                             const FewArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  FewSmem<MN>& sm = *reinterpret_cast<FewSmem<MN>*>(smem_raw + pad);
+  DevStatus* status = &g_matmul_status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ranks = cluster_size(), rank = cluster_rank();
+  const int tile = blockIdx.x / ranks;
+  // this CTA's k-blocks
+  const int k0 = static_cast<int>(static_cast<int64_t>(a.kb) * rank / ranks);
+  const int nk = static_cast<int>(static_cast<int64_t>(a.kb) * (rank + 1) / ranks) - k0;
+  constexpr uint32_t kCols = 2 * MN < 32 ? 32 : 2 * MN;
+  if (tid == 0) {
+    sm.abort = 0;
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.t_full[b], 1);
+      mbar_init(&sm.t_empty[b], 4);
+    }
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, kCols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = sm.tmem_base;
+  volatile int* abort = &sm.abort;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_w);
+      prefetch_tmap(&tm_x);
+      int it = 0;
+      bool ok = true;
+      for (; it < nk; ++it) {
+        const int s = it % kFewStages;
+        if (it >= kFewStages && !(ok = mbar_wait(&sm.empty[s], ((it / kFewStages) + 1) & 1, abort, status, 11))) break;
+        mbar_expect_tx(&sm.full[s], (128 + MN) * kBK);
+        tma_load_2d(sm.w[s], &tm_w, (k0 + it) * kBK, tile * 128, &sm.full[s]);
+        tma_load_2d(sm.x[s], &tm_x, (k0 + it) * kBK, 0, &sm.full[s]);
+      }
+      if (!ok || *abort) {
+        for (int j = max(0, it - kFewStages); j < it; ++j) {
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&sm.full[j % kFewStages], (j / kFewStages) & 1) && clock64() - t0 < kWaitCycles / 4) {
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const uint32_t leader = elect_one();
+    constexpr uint32_t idesc = idesc_e4m3(128, MN, false);
+    for (int it = 0; it < nk; ++it) {
+      const int s = it % kFewStages, b = it & 1;
+      if (it >= 2 && !mbar_wait(&sm.t_empty[b], ((it >> 1) + 1) & 1, abort, status, 12)) break;
+      if (!mbar_wait(&sm.full[s], (it / kFewStages) & 1, abort, status, 13)) break;
+      tc_fence_after();
+      const uint32_t wa = smem_u32(sm.w[s]), xa = smem_u32(sm.x[s]);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        mma_f8_if(tbase + b * MN, desc_kmajor(wa + kk * 32), desc_kmajor(xa + kk * 32), idesc, kk > 0, leader);
+      tc_commit_if(&sm.t_full[b], leader);
+      tc_commit_if(&sm.empty[s], leader);
+    }
+    tc_commit_if(&sm.drain, leader);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(&sm.drain, 0) && clock64() - t0 < kWaitCycles) {
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int wq = warp & 3, row = wq * 32 + lane;   // weight row of the tile
+    const uint32_t lb = tbase + (static_cast<uint32_t>(wq * 32) << 16);
+    const int p = tid - 128;
+    // thread p < MN brings the scale of activation row p, one block ahead
+    const float* sa = a.sa + static_cast<int64_t>(min(p, a.M - 1)) * a.sam + k0 * a.sak;
+    const float* sb = a.sb + static_cast<int64_t>(tile) * a.sbn + k0 * a.sbk;
+    float acc[MN], xs = 0.f, ys = 0.f;
+    bool ok = true;
+#pragma unroll
+    for (int c = 0; c < MN; ++c) acc[c] = 0.f;
+    if (p < MN && nk > 0) {
+      xs = __ldg(sa);
+      ys = __ldg(sb);
+    }
+    for (int it = 0; it < nk; ++it) {
+      const int b = it & 1;
+      if (p < MN) {
+        sm.scale[b][p] = xs * ys;
+        if (it + 1 < nk) {
+          xs = __ldg(sa + (it + 1) * a.sak);
+          ys = __ldg(sb + (it + 1) * a.sbk);
+        }
+      }
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");   // the scales of this block are written, those of it - 1 read
+      // (a warp that gave up keeps step with the others' barrier)
+      ok = ok && mbar_wait(&sm.t_full[b], (it >> 1) & 1, abort, status, 14);
+      tc_fence_after();
+      float x[MN];
+#pragma unroll
+      for (int c = 0; c < MN; c += 16) tmem_ld16(lb + b * MN + c, *reinterpret_cast<float(*)[16]>(x + c));
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < MN; c += 16) reg_fence16(*reinterpret_cast<float(*)[16]>(x + c));
+      tc_fence_before();
+      warp_arrive(&sm.t_empty[b], lane);
+#pragma unroll
+      for (int c = 0; c < MN; c += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(&sm.scale[b][c]);
+        fma2(acc[c], acc[c + 1], x[c], x[c + 1], s.x, s.y);
+        fma2(acc[c + 2], acc[c + 3], x[c + 2], x[c + 3], s.z, s.w);
+      }
+    }
+#pragma unroll
+    // (every MMA has read its weights: t_full of the last block is through)
+    for (int c = 0; c < MN; ++c) reinterpret_cast<float*>(sm.w)[c * 128 + row] = acc[c];
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tbase, kCols);
+  cluster_sync();
+  // each rank adds the parts of its share of the (row, column) pairs, columns fastest
+  const int all = min(MN, a.M) * 128;
+  const bool dead = *abort != 0;
+  for (int i = rank * 256 + tid; i < all && !dead; i += ranks * 256) {
+    const int m = i >> 7, c = i & 127, n = tile * 128 + c;
+    if (n >= a.N) continue;
+    float v = 0.f, part[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) part[r] = r < ranks ? ld_cluster(reinterpret_cast<const float*>(sm.w) + i, r) : 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v += part[r];
+    if (a.bias != nullptr) v += __ldg(a.bias + n);
+    const int64_t o = static_cast<int64_t>(m) * a.ldo + n;
+    store1<ODT>(a.out, o, v);
+  }
+  __syncwarp();
+  cluster_sync();   // no CTA leaves while another reads its part
 }
 
 // ---- host side ---------------------------------------------------------------
@@ -339,8 +596,26 @@ struct Operands {
   int64_t lda, ldb, K;
 };
 
-template <int BN, int ODT>
-cudaError_t launch(const Operands& op, MatmulArgs a, cudaStream_t st) {
+template <typename K, typename A>
+cudaError_t launch_cluster(K kernel, unsigned ctas, int threads, int smem, int ranks, cudaStream_t st,
+                           const CUtensorMap& m0, const CUtensorMap& m1, const A& a) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, m0, m1, a);
+}
+
+template <int BN, int ODT, bool SPLIT>
+cudaError_t launch(const Operands& op, MatmulArgs a, int ranks, cudaStream_t st) {
   CUtensorMap ma, mb;
   if (!make_map(&ma, op.a, a.M, op.K, op.lda, kBM) || !make_map(&mb, op.b, a.N, op.K, op.ldb, BN))
     return cudaErrorInvalidValue;
@@ -348,20 +623,50 @@ cudaError_t launch(const Operands& op, MatmulArgs a, cudaStream_t st) {
   a.nt = (a.N + BN - 1) / BN;
   a.tiles = a.mt * a.nt;
   a.group = 16;
-  auto k = matmul_blocks_kernel<BN, ODT>;
+  a.ranks = ranks;
+  auto k = matmul_blocks_kernel<BN, ODT, SPLIT>;
   const int smem = static_cast<int>(sizeof(MmSmem<BN>)) + 1024;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  k<<<static_cast<unsigned>(min(a.tiles, sm_count())), MmCfg<BN>::kThreads, smem, st>>>(ma, mb, a);
-  return cudaGetLastError();
+  if constexpr (!SPLIT) {
+    k<<<static_cast<unsigned>(min(a.tiles, sm_count())), MmCfg<BN>::kThreads, smem, st>>>(ma, mb, a);
+    return cudaGetLastError();
+  }
+  return launch_cluster(k, static_cast<unsigned>(a.tiles) * ranks, MmCfg<BN>::kThreads, smem, ranks, st, ma, mb, a);
+}
+
+template <int MN, int ODT>
+cudaError_t launch_few(const Operands& op, const MatmulArgs& m, cudaStream_t st) {
+  CUtensorMap mw, mx;
+  if (!make_map(&mw, op.b, m.N, op.K, op.ldb, 128) || !make_map(&mx, op.a, m.M, op.K, op.lda, MN))
+    return cudaErrorInvalidValue;
+  FewArgs a{m.sa, m.sb, m.sam, m.sak, m.sbn, m.sbk, m.bias, m.out, m.ldo, m.M, m.N, m.kb};
+  auto k = matmul_blocks_few_kernel<MN, ODT>;
+  const int smem = static_cast<int>(sizeof(FewSmem<MN>)) + 1024;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  // CTAs per row tile: enough for the CTAs that fit on every SM, at least two k-blocks each
+  const int tiles = (m.N + 127) / 128;
+  const int want = ((MN == 16 ? 3 : 2) * sm_count()) / tiles;
+  const int ranks = max(1, min(min(8, want), m.kb / 2));
+  return launch_cluster(k, static_cast<unsigned>(tiles) * ranks, 256, smem, ranks, st, mw, mx, a);
 }
 
 template <int ODT>
 cudaError_t dispatch(const Operands& op, const MatmulArgs& a, cudaStream_t st) {
-  // 256-column tiles halve the A traffic per MMA; with too few tiles to fill
-  // the SMs the narrower tile spreads the work further.
-  const int64_t wide = static_cast<int64_t>((a.M + 127) / 128) * ((a.N + 255) / 256);
-  return wide >= sm_count() ? launch<256, ODT>(op, a, st) : launch<128, ODT>(op, a, st);
+  // Few rows: the kernel that streams the weight (N = 7168, K = 5376: M = 32 in
+  // 12.7 us against 16.7 with 128-row tiles; at M = 64 it would take 21 us).
+  if (a.M <= 16) return launch_few<16, ODT>(op, a, st);
+  if (a.M <= 32) return launch_few<32, ODT>(op, a, st);
+  // A 256-column tile reads half the A bytes per MMA, a 128-column tile of the
+  // same k-block takes 0.55 of its time: the one with the shorter run of whole
+  // tiles on the busiest SM.
+  const int64_t sms = sm_count(), mt = (a.M + 127) / 128;
+  const int64_t t256 = mt * ((a.N + 255) / 256), t128 = mt * ((a.N + 127) / 128);
+  if (20 * ((t256 + sms - 1) / sms) <= 11 * ((t128 + sms - 1) / sms)) return launch<256, ODT, false>(op, a, 1, st);
+  // Tiles for less than half of the SMs: clusters share their k-blocks.
+  const int ranks = static_cast<int>(min(min(sms / t128, int64_t{8}), static_cast<int64_t>(a.kb / 4)));
+  return ranks >= 2 ? launch<128, ODT, true>(op, a, ranks, st) : launch<128, ODT, false>(op, a, 1, st);
 }
 
 int arg_error(const char* msg) {
