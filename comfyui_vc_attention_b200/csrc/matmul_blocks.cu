@@ -8,7 +8,8 @@
 // runs.  Thread = output row (TMEM lane) and 64 columns, so the scale of a
 // block is one scalar per thread.
 //   warp 0       TMA producer        warp 1   MMA issuer, tensor-memory owner
-//   warps 2-3    sa * sb of each k-block into a ring in shared memory
+//   warps 2-3    sa * sb of four k-blocks at a time, in two groups in shared
+//                memory, the next group's loads in flight
 //   warps 4-     promotion and output
 #include <cuda.h>
 #include <mutex>
@@ -77,15 +78,15 @@ template <int ODT> __device__ __forceinline__ void store1(void* out, int64_t i, 
   else static_cast<float*>(out)[i] = v;
 }
 
-constexpr int kScales = 8;   // k-blocks that the scale ring holds
+constexpr int kGroup = 4;   // k-blocks whose scales change hands together (two groups in shared memory)
 
 template <int BN> struct MmCfg {
   static constexpr int kStages = BN == 256 ? 3 : 5;
   static constexpr int kPromo = BN / 64 * 4;               // promotion warps
   static constexpr int kThreads = 128 + 32 * kPromo;
   static constexpr int kTmemCols = 2 * BN;
-  // Output staging of a warp: 32 rows of 64 16-bit values (or 32 fp32 values),
-  // 16 bytes apart more than their length so that the rows start in different banks.
+  // Output staging of a warp: 32 bytes of each of its 32 rows at a time, 16
+  // bytes apart so that the rows start in different banks.
   static constexpr int kOutPitch = 128 + 16;
   static constexpr int kPartPitch = BN + 4;   // floats of a row of a rank's sums
   static_assert(kBM * kPartPitch * 4 <= kStages * kBM * kBK + kStages * BN * kBK, "a rank's sums fit over the stages");
@@ -95,13 +96,13 @@ template <int BN> struct MmSmem {
   alignas(1024) uint8_t a[MmCfg<BN>::kStages][kBM * kBK];
   alignas(1024) uint8_t b[MmCfg<BN>::kStages][BN * kBK];
   alignas(16) uint8_t out[MmCfg<BN>::kPromo][32 * MmCfg<BN>::kOutPitch];
-  alignas(16) float scale[kScales][BN / 128][kBM];
+  alignas(16) float scale[2][BN / 128][kBM][kGroup];
   alignas(8) uint64_t full[MmCfg<BN>::kStages];
   alignas(8) uint64_t empty[MmCfg<BN>::kStages];
   alignas(8) uint64_t t_full[2];
   alignas(8) uint64_t t_empty[2];
-  alignas(8) uint64_t s_full[kScales];
-  alignas(8) uint64_t s_empty[kScales];
+  alignas(8) uint64_t s_full[2];
+  alignas(8) uint64_t s_empty[2];
   alignas(8) uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -137,10 +138,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.t_full[b], 1);
       mbar_init(&sm.t_empty[b], Cfg::kPromo);
-    }
-    for (int r = 0; r < kScales; ++r) {
-      mbar_init(&sm.s_full[r], 2);
-      mbar_init(&sm.s_empty[r], Cfg::kPromo);
+      mbar_init(&sm.s_full[b], 2);
+      mbar_init(&sm.s_empty[b], Cfg::kPromo);
     }
     mbar_init(&sm.drain, 1);
     fence_mbar_init();
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   } else {
     // ------------------------------------------------------------ scales
     const int r = tid - 64;   // rows r and r + 64
-    int it = 0;
+    int grp = 0;              // groups handed over
     bool ok = true;
     for (int t = t0; ok && t < a.tiles; t += t_step) {
       int mt, nt;
@@ -226,34 +225,31 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       // (rows and columns past the matrix take the scale of the last one: nothing of them is written)
       const float* sa0 = a.sa + static_cast<int64_t>(min(mt * kBM + r, a.M - 1)) * a.sam;
       const float* sa1 = a.sa + static_cast<int64_t>(min(mt * kBM + r + 64, a.M - 1)) * a.sam;
-      const float* sb[BN / 128];
+      const float* sb = a.sb + static_cast<int64_t>(nt) * (BN / 128) * a.sbn;
+      const int64_t sb1 = (nt * BN + 128 < a.N) ? a.sbn : 0;
+      float x0[kGroup], x1[kGroup], y0[kGroup], y1[kGroup];
+      auto load = [&](int k) {
 #pragma unroll
-      for (int c = 0; c < BN / 128; ++c) sb[c] = a.sb + static_cast<int64_t>(min(nt * BN + c * 128, a.N - 1) / 128) * a.sbn;
-      for (int k0 = kb0; ok && k0 < kb1; k0 += 4) {
-        // four blocks' scales in flight
-        float x0[4], x1[4], y[4][BN / 128];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int k = min(k0 + u, kb1 - 1);
-          x0[u] = __ldg(sa0 + k * a.sak);
-          x1[u] = __ldg(sa1 + k * a.sak);
-#pragma unroll
-          for (int c = 0; c < BN / 128; ++c) y[u][c] = __ldg(sb[c] + k * a.sbk);
+        for (int u = 0; u < kGroup; ++u) {
+          const int kk = min(k + u, kb1 - 1);
+          x0[u] = __ldg(sa0 + kk * a.sak);
+          x1[u] = __ldg(sa1 + kk * a.sak);
+          y0[u] = __ldg(sb + kk * a.sbk);
+          if constexpr (BN == 256) y1[u] = __ldg(sb + sb1 + kk * a.sbk);
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (ok && k0 + u < kb1) {
-            const int s = it % kScales;
-            if (it >= kScales) ok = mbar_wait(&sm.s_empty[s], ((it / kScales) + 1) & 1, abort, status, 5);
-#pragma unroll
-            for (int c = 0; c < BN / 128; ++c) {
-              sm.scale[s][c][r] = x0[u] * y[u][c];
-              sm.scale[s][c][r + 64] = x1[u] * y[u][c];
-            }
-            warp_arrive(&sm.s_full[s], lane);
-            ++it;
-          }
+      };
+      load(kb0);
+      for (int k = kb0; k < kb1; k += kGroup, ++grp) {
+        const int s = grp & 1;
+        if (grp >= 2 && !(ok = mbar_wait(&sm.s_empty[s], ((grp >> 1) + 1) & 1, abort, status, 5))) break;
+        *reinterpret_cast<float4*>(sm.scale[s][0][r]) = make_float4(x0[0] * y0[0], x0[1] * y0[1], x0[2] * y0[2], x0[3] * y0[3]);
+        *reinterpret_cast<float4*>(sm.scale[s][0][r + 64]) = make_float4(x1[0] * y0[0], x1[1] * y0[1], x1[2] * y0[2], x1[3] * y0[3]);
+        if constexpr (BN == 256) {
+          *reinterpret_cast<float4*>(sm.scale[s][1][r]) = make_float4(x0[0] * y1[0], x0[1] * y1[1], x0[2] * y1[2], x0[3] * y1[3]);
+          *reinterpret_cast<float4*>(sm.scale[s][1][r + 64]) = make_float4(x1[0] * y1[0], x1[1] * y1[1], x1[2] * y1[2], x1[3] * y1[3]);
         }
+        warp_arrive(&sm.s_full[s], lane);
+        if (k + kGroup < kb1) load(k + kGroup);   // in flight while the promotion works on this group
       }
     }
   }
@@ -264,7 +260,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const uint32_t lb = tbase + (static_cast<uint32_t>(wq * 32) << 16) + quarter * 64;
     constexpr int ES = ODT == VCATTN_DTYPE_F32 ? 4 : 2;
     uint8_t* stage = sm.out[warp - 4];
-    int it = 0;
+    const float* scale = sm.scale[0][quarter >> 1][wq * 32 + lane];
+    uint32_t b = 0, b_par = 0, g = 0, g_par = 0;   // tensor-memory buffer and scale group, and their phases
     bool ok = true;
     for (int t = t0; ok && t < a.tiles; t += t_step) {
       int mt, nt;
@@ -273,27 +270,32 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       float acc[64];
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-      for (int k = kb0; k < kb1; ++k, ++it) {
-        const int b = it & 1, r = it % kScales;
-        if (!(ok = mbar_wait2(&sm.s_full[r], (it / kScales) & 1, &sm.t_full[b], (it >> 1) & 1, abort, status, 4))) break;
-        const float s = sm.scale[r][quarter >> 1][wq * 32 + lane];
-        tc_fence_after();
+      for (int k = kb0; ok && k < kb1; k += kGroup) {
+        if (!(ok = mbar_wait(&sm.s_full[g], g_par, abort, status, 4))) break;
+        const float4 s4 = *reinterpret_cast<const float4*>(scale + g * (BN / 128 * kBM * kGroup));
+        warp_arrive(&sm.s_empty[g], lane);
+        g ^= 1;
+        g_par ^= g ^ 1;   // (flips when g returns to 0)
+        const float s[kGroup] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[32];
-          tmem_ld32(lb + b * BN + h * 32, x);
-          tmem_ld_wait();
-          reg_fence(x);
-          if (h == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&sm.t_empty[b]);
-              mbar_arrive(&sm.s_empty[r]);
+        for (int u = 0; u < kGroup; ++u) {
+          if (k + u >= kb1 || !(ok = mbar_wait(&sm.t_full[b], b_par, abort, status, 6))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            tmem_ld32(lb + b * BN + h * 32, x);
+            tmem_ld_wait();
+            reg_fence(x);
+            if (h == 1) {
+              tc_fence_before();
+              warp_arrive(&sm.t_empty[b], lane);
             }
-          }
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) fma2(acc[h * 32 + c], acc[h * 32 + c + 1], x[c], x[c + 1], s, s);
+            for (int c = 0; c < 32; c += 2) fma2(acc[h * 32 + c], acc[h * 32 + c + 1], x[c], x[c + 1], s[u], s[u]);
+          }
+          b ^= 1;
+          b_par ^= b ^ 1;
         }
       }
       if (!ok || *abort) continue;
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         for (int c = 0; c < 64; c += 4) *reinterpret_cast<float4*>(part + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
         continue;
       }
-      // rows through shared memory, so that whole 128-byte lines go out
+      // rows through shared memory, so that whole 32-byte sectors go out
       constexpr int PC = 128 / ES;   // columns per pass
 #pragma unroll
       for (int p = 0; p < 64 / PC; ++p) {
@@ -324,9 +326,9 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
           *reinterpret_cast<uint4*>(stage + lane * Cfg::kOutPitch + c * ES) = w;
         }
         __syncwarp();
-        const int cols = min(PC, a.N - np);
-        for (int i = lane; i < 32 * 8; i += 32) {
-          const int r = i >> 3, c = (i & 7) * (16 / ES);   // 16-byte chunk of a row
+        const int c = (lane & 7) * (16 / ES), cols = a.N - np;   // 16-byte chunk of a row
+#pragma unroll
+        for (int r = lane >> 3; r < 32; r += 4) {
           if (m0 + r >= a.M || c >= cols) continue;
           const uint8_t* src = stage + r * Cfg::kOutPitch + c * ES;
           uint8_t* dst = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(m0 + r) * a.ldo + np + c) * ES;

@@ -4,12 +4,16 @@
 // Blocks are 1 x 128 (activations: one scale per row) or 128 x 128 (weights).
 // A NaN in a block makes its scale, and so the whole block, NaN.
 //
-// Sixteen lanes hold one 128-column row segment, eight columns each.  Bound by
-// HBM: the elements are read once and stay in registers over the maximum and
-// the conversion.
+// Sixteen lanes hold one 128-column row segment, eight columns each, in
+// registers as loaded: the maximum is taken on the 16-bit pairs.  Both
+// quotients are Markstein's correction of a product with the reciprocal (see
+// DivBy), so the scales and codes are those of IEEE divisions; the one of x / s
+// runs on packed fp32 pairs.  Bound by HBM where the instructions allow: the
+// elements are read once.
 #include <string>
 
 #include "kernels.cuh"
+#include "tc_math.cuh"
 
 namespace vcattn {
 namespace {
@@ -35,66 +39,125 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// Eight columns from c on of one row (columns past K read as 0).
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_cols(const QuantArgs& a, int64_t row, int c, float (&v)[8]) {
-  using T = typename Elem<DT>::T;
-  const T* p = static_cast<const T*>(a.x) + row * a.ldx + c;
-  if (VEC && c + 8 <= a.K) {
-    if constexpr (DT == VCATTN_DTYPE_F32) {
-      const float4 f = load4<DT>(p, 0), g = load4<DT>(p, 4);
-      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-      v[4] = g.x; v[5] = g.y; v[6] = g.z; v[7] = g.w;
+// Eight consecutive columns as loaded: 16-bit pairs, or fp32.
+template <int DT> struct Cols8 {
+  uint32_t u[4];
+  __device__ __forceinline__ float max_abs() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max_pair(m, u[i] & 0x7fff7fffu);
+    if constexpr (DT == VCATTN_DTYPE_BF16) return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+    return max_nan(f.x, f.y);
+  }
+  // Per half, NaN if either is.
+  static __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    if constexpr (DT == VCATTN_DTYPE_BF16) {
+      const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&r);
     } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const uint32_t r[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (DT == VCATTN_DTYPE_BF16) {
-          v[2 * i] = __uint_as_float(r[i] << 16);
-          v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-        } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-          v[2 * i] = f.x;
-          v[2 * i + 1] = f.y;
-        }
-      }
+      const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&r);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < a.K ? Elem<DT>::load(p + i) : 0.f;
   }
-}
-
-__device__ __forceinline__ float max8(const float (&v)[8]) {
-  float m = fabsf(v[0]);
+  __device__ __forceinline__ void pair(int i, float& x, float& y) const {
+    if constexpr (DT == VCATTN_DTYPE_BF16) {
+      x = __uint_as_float(u[i] << 16);
+      y = __uint_as_float(u[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x = f.x;
+      y = f.y;
+    }
+  }
+  __device__ __forceinline__ void load(const void* p) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
+  }
+  __device__ __forceinline__ void load_some(const void* p, int n) {
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
-  return m;
+    for (int i = 0; i < 4; ++i) {
+      u[i] = 2 * i < n ? static_cast<const uint16_t*>(p)[2 * i] : 0u;
+      if (2 * i + 1 < n) u[i] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[2 * i + 1]) << 16;
+    }
+  }
+};
+template <> struct Cols8<VCATTN_DTYPE_F32> {
+  float v[8];
+  __device__ __forceinline__ float max_abs() const {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+    return m;
+  }
+  __device__ __forceinline__ void pair(int i, float& x, float& y) const {
+    x = v[2 * i];
+    y = v[2 * i + 1];
+  }
+  __device__ __forceinline__ void load(const void* p) {
+    const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  __device__ __forceinline__ void load_some(const void* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? static_cast<const float*>(p)[i] : 0.f;
+  }
+};
+
+// Eight columns from c on of one row (columns past K, or all if !in, read as 0).
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_cols(const QuantArgs& a, bool in, int64_t row, int c, Cols8<DT>& v) {
+  const int n = in ? a.K - c : 0;
+  const void* p = static_cast<const typename Elem<DT>::T*>(a.x) + (n > 0 ? row * a.ldx + c : 0);
+  if (VEC && n >= 8) v.load(p);
+  else v.load_some(p, n);
 }
 
-__device__ __forceinline__ float block_scale(float amax) { return __fdiv_rn(max_nan(amax, kTiny), kE4M3Max); }
+// max(amax, 1e-30) / 448: Markstein's quotient with the constant's reciprocal.
+__device__ __forceinline__ float block_scale(float amax) {
+  amax = max_nan(amax, kTiny);
+  constexpr float y = 1.0f / kE4M3Max;
+  const float q0 = __fmul_rn(amax, y);
+  const float q = __fmaf_rn(__fmaf_rn(-q0, kE4M3Max, amax), y, q0);
+  return amax < INFINITY ? q : amax;
+}
 
-// Codes of eight columns (the columns past K are not written).  The quotient
-// is DivBy's; an infinite or NaN scale takes the division itself.
-__device__ __forceinline__ void store_codes(const QuantArgs& a, int64_t row, int c, const float (&v)[8], float s) {
-  float q[8];
+__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Codes of eight columns (the columns past K are not written).
+template <int DT>
+__device__ __forceinline__ void store_codes(const QuantArgs& a, int64_t row, int c, const Cols8<DT>& v, float s, float y) {
+  uint32_t w[4];
   if (s < INFINITY) {
-    const DivBy by(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = by(v[i]);
-  } else {
+    for (int i = 0; i < 4; ++i) {
+      float x0, x1;
+      v.pair(i, x0, x1);
+      float q0 = x0, q1 = x1;
+      tc::mul2(q0, q1, y, y);
+      tc::fma2(x0, x1, q0, q1, -s, -s);   // the remainder
+      tc::fma2(q0, q1, x0, x1, y, y);
+      w[i] = codes2(q0, q1);
+    }
+  } else {   // an infinite or NaN block: the divisions themselves
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i], s);
+    for (int i = 0; i < 4; ++i) {
+      float x0, x1;
+      v.pair(i, x0, x1);
+      w[i] = codes2(__fdiv_rn(x0, s), __fdiv_rn(x1, s));
+    }
   }
-  const uint2 w = make_uint2(e4m3x4(q[0], q[1], q[2], q[3]), e4m3x4(q[4], q[5], q[6], q[7]));
+  const uint2 b = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
   uint8_t* p = a.codes + row * a.ldc + c;
   if (c + 8 <= a.K) {   // ldc and the base are multiples of 16
-    *reinterpret_cast<uint2*>(p) = w;
+    *reinterpret_cast<uint2*>(p) = b;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < a.K) p[i] = static_cast<uint8_t>((i < 4 ? w.x >> (8 * i) : w.y >> (8 * (i - 4))) & 0xffu);
+      if (c + i < a.K) p[i] = static_cast<uint8_t>(((i < 4 ? b.x : b.y) >> (8 * (i & 3))) & 0xffu);
   }
 }
 
@@ -105,11 +168,14 @@ template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) quant_rows_blocks_kernel(const QuantArgs a) {
   const int l = threadIdx.x & 15;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4)) * kSegs;
-  float v[kSegs][8];
+  Cols8<DT> v[kSegs];
   int64_t row[kSegs];
   int blk[kSegs];
   {
-    int64_t r = first / a.kb;
+    // (a 64-bit division takes longer than the rest of the block)
+    int64_t r;
+    if (a.segs < (int64_t{1} << 31)) r = static_cast<uint32_t>(first) / static_cast<uint32_t>(a.kb);
+    else r = first / a.kb;
     int b = static_cast<int>(first - r * a.kb);
 #pragma unroll
     for (int u = 0; u < kSegs; ++u) {
@@ -122,21 +188,16 @@ __global__ void __launch_bounds__(kThreads) quant_rows_blocks_kernel(const Quant
     }
   }
 #pragma unroll
-  for (int u = 0; u < kSegs; ++u) {
-    if (first + u < a.segs) load_cols<DT, VEC>(a, row[u], blk[u] * kBlk + l * 8, v[u]);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-  }
+  for (int u = 0; u < kSegs; ++u) load_cols<DT, VEC>(a, first + u < a.segs, row[u], blk[u] * kBlk + l * 8, v[u]);
 #pragma unroll
   for (int u = 0; u < kSegs; ++u) {
-    float m = max8(v[u]);
+    float m = v[u].max_abs();
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (first + u < a.segs) {
       const float s = block_scale(m);
       if (l == 0) a.scale[row[u] * a.ssm + blk[u] * a.ssk] = s;
-      store_codes(a, row[u], blk[u] * kBlk + l * 8, v[u], s);
+      store_codes<DT>(a, row[u], blk[u] * kBlk + l * 8, v[u], s, __frcp_rn(s));
     }
   }
 }
@@ -149,28 +210,23 @@ __global__ void __launch_bounds__(kThreads) quant_square_blocks_kernel(const Qua
   const int blk = static_cast<int>(blockIdx.x - mb * a.kb);
   const int c = blk * kBlk + (threadIdx.x & 15) * 8;
   const int64_t r0 = mb * kBlk + (threadIdx.x >> 4);
-  float v[8][8];
+  Cols8<DT> v[8];
   float m = 0.f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    if (r0 + 16 * u < a.M) load_cols<DT, VEC>(a, r0 + 16 * u, c, v[u]);
-    else
+  for (int u = 0; u < 8; ++u) load_cols<DT, VEC>(a, r0 + 16 * u < a.M, r0 + 16 * u, c, v[u]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-  }
-#pragma unroll
-  for (int u = 0; u < 8; ++u) m = max_nan(m, max8(v[u]));
+  for (int u = 0; u < 8; ++u) m = max_nan(m, v[u].max_abs());
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) m = max_nan(m, wmax[w]);
-  const float s = block_scale(m);
+  const float s = block_scale(m), y = __frcp_rn(s);
   if (threadIdx.x == 0) a.scale[mb * a.ssm + blk * a.ssk] = s;
 #pragma unroll
   for (int u = 0; u < 8; ++u)
-    if (r0 + 16 * u < a.M) store_codes(a, r0 + 16 * u, c, v[u], s);
+    if (r0 + 16 * u < a.M) store_codes<DT>(a, r0 + 16 * u, c, v[u], s, y);
 }
 
 template <int DT, bool VEC>
