@@ -4,22 +4,26 @@
 //   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s)   on the first `rot` channels
 // with j = i + rot/2 (half layout) or j = i + 1, i even (interleaved).
 //
-// A row is spread over LPR lanes, eight channels each (one 16-byte load for
-// 16-bit types).  Since the norm is one factor per row, w, cos and sin fold
-// into two coefficients per channel, out_e = r * (x_e cw_e + x_p sw_e) with p
-// the partner channel; a warp keeps them in registers while it walks over
-// heads of one token, so the table is read once per group of heads.  In the
-// half layout the partner's raw channels come from another lane of the row.
-// Bound by HBM: every element is read once and written once.
+// A row is spread over LPR lanes in chunks of eight channels (16-byte loads for
+// 16-bit types): one chunk per lane in the interleaved layout, two in the half
+// layout, where they are partners, so no channel crosses lanes.  Since the norm is one factor per row,
+// w, cos and sin fold into two coefficients per channel,
+// out_e = r * (x_e cw_e + x_p sw_e) with p the partner channel; a warp makes
+// them for one token and applies them to its heads, whose rows it has loaded
+// before.  Bound by HBM, every element read once and written once; the packed
+// fp32 arithmetic keeps the instructions (about five per element) below that.
 #include <string>
 
 #include "kernels.cuh"
+#include "tc_math.cuh"
 
 namespace vcattn {
 namespace {
 
-constexpr int kWarpsPerCta = 8;
-constexpr int kRowsInFlight = 4;   // loads issued per lane before the first use
+constexpr int kWarpsPerCta = 4;
+// Rows loaded per lane before the first use (16384 x 112 rows of 128 bf16, 96
+// rotated: 2, 3 and 4 rows in the half layout take 175, 170 and 183 us).
+template <bool HALF> constexpr int kRowsInFlight = HALF ? 3 : 4;
 
 struct RopeArgs {
   const void* x[2];
@@ -58,14 +62,6 @@ template <int DT> struct Raw8 {
       }
     }
   }
-  __device__ __forceinline__ Raw8 from_lane(int src) const {
-    Raw8 o;
-    o.u.x = __shfl_sync(0xffffffffu, u.x, src);
-    o.u.y = __shfl_sync(0xffffffffu, u.y, src);
-    o.u.z = __shfl_sync(0xffffffffu, u.z, src);
-    o.u.w = __shfl_sync(0xffffffffu, u.w, src);
-    return o;
-  }
   static __device__ __forceinline__ void store(void* base, int64_t off, const float (&v)[8]) {
     uint32_t r[4];
 #pragma unroll
@@ -93,16 +89,6 @@ template <> struct Raw8<VCATTN_DTYPE_F32> {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
-  __device__ __forceinline__ Raw8 from_lane(int src) const {
-    float v[8];
-    values(v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], src);
-    Raw8 o;
-    o.a = make_float4(v[0], v[1], v[2], v[3]);
-    o.b = make_float4(v[4], v[5], v[6], v[7]);
-    return o;
-  }
   static __device__ __forceinline__ void store(void* base, int64_t off, const float (&v)[8]) {
     float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + off);
     p[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -119,10 +105,10 @@ __device__ __forceinline__ void load8f(const float* p, float (&v)[8]) {
 template <int DT, int LPR, bool HALF>
 __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rope_kernel(const RopeArgs a) {
   constexpr int RPW = 32 / LPR;   // rows (heads) side by side in a warp
+  constexpr int CH = HALF ? 2 : 1, U = kRowsInFlight<HALF>;
   const uint32_t item = blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
   if (item >= a.items) return;    // whole warps
-  const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR, e0 = l * 8;
-  const bool live = e0 < a.D;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR;
   const uint32_t tokens = static_cast<uint32_t>(a.B) * a.N;
   const uint32_t tok = a.token_major ? item / a.chunks : item % tokens;
   const int chunk = a.token_major ? item % a.chunks : item / tokens;
@@ -131,109 +117,135 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) qk_norm_rope_kernel(const R
   const int h0 = (t ? chunk - a.chunks_q : chunk) * a.chunk_heads;
   const int h1 = min(h0 + a.chunk_heads, a.heads[t]);
 
-  // coefficients of this lane's channels
-  float cw[8], sw[8];
-  const bool turned = e0 < a.rot;
-  const int half = a.rot >> 1;
-  const int pl = !HALF || !turned ? l : (e0 < half ? l + half / 8 : l - half / 8);   // partner's lane in the row
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cw[i] = 1.f;
-    sw[i] = 0.f;
+  // This lane's first channels: in the half layout chunk l of the first
+  // rotated half and its partner, then the channels past `rot` in two halves.
+  const int row_chunks = a.D / 8;
+  const int pairs = HALF ? a.rot / 16 : 0;
+  const int rest = HALF ? (row_chunks - 2 * pairs + 1) / 2 : row_chunks;
+  const bool partner = l < pairs;
+  int e[CH];
+  bool live[CH];
+  e[0] = 8 * (partner ? l : pairs + l);                    // (2 pairs + (l - pairs))
+  live[0] = l < pairs + rest;
+  if constexpr (HALF) {
+    e[1] = 8 * (partner ? pairs + l : pairs + rest + l);
+    live[1] = live[0] && e[1] < a.D;
   }
-  if (live) {
-    float wp[8];
+
+  const int64_t xoff = b * a.xsb[t] + n * a.xsn[t], yoff = b * a.ysb[t] + n * a.ysn[t];
+  Raw8<DT> raw[U][CH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) wp[i] = 1.f;
-    if (a.w[t] != nullptr) {
-      load8f(a.w[t] + e0, cw);
-      load8f(a.w[t] + pl * 8, wp);
+  for (int u = 0; u < U; ++u) {   // in flight while the coefficients are made
+    const int h = h0 + u * RPW + sub;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (live[j] && h < h1) raw[u][j].load(a.x[t], xoff + h * a.xsh[t] + e[j]);
+      else raw[u][j].zero();
     }
-    if (turned) {
-      const int64_t row = b * a.tsb + n * a.tsn;
-      if constexpr (HALF) {
-        const bool lower = e0 < half;
-        float c[8], s[8];
-        load8f(a.cos + row + (lower ? e0 : e0 - half), c);
-        load8f(a.sin + row + (lower ? e0 : e0 - half), s);
+  }
+
+  float cw[CH][8], sw[CH][8];
+  bool turned[CH];
+  const int64_t trow = b * a.tsb + n * a.tsn;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          cw[i] *= c[i];
-          sw[i] = wp[i] * (lower ? -s[i] : s[i]);
-        }
-      } else {
-        const float4 c = *reinterpret_cast<const float4*>(a.cos + row + e0 / 2);
-        const float4 s = *reinterpret_cast<const float4*>(a.sin + row + e0 / 2);
+  for (int j = 0; j < CH; ++j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cw[j][i] = 1.f;
+    if (live[j] && a.w[t] != nullptr) load8f(a.w[t] + e[j], cw[j]);
+    turned[j] = HALF ? partner : live[j] && e[j] < a.rot;
+  }
+  if constexpr (HALF) {
+    if (partner) {
+      float c[8], s[8];
+      load8f(a.cos + trow + e[0], c);
+      load8f(a.sin + trow + e[0], s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sw[0][i] = -cw[1][i] * s[i];
+        sw[1][i] = cw[0][i] * s[i];
+        cw[0][i] *= c[i];
+        cw[1][i] *= c[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (turned[j]) {
+        const float4 c = *reinterpret_cast<const float4*>(a.cos + trow + e[j] / 2);
+        const float4 s = *reinterpret_cast<const float4*>(a.sin + trow + e[j] / 2);
         const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sw[2 * i] = -wp[2 * i + 1] * ss[i];
-          sw[2 * i + 1] = wp[2 * i] * ss[i];
-          cw[2 * i] *= cc[i];
-          cw[2 * i + 1] *= cc[i];
+          sw[j][2 * i] = -cw[j][2 * i + 1] * ss[i];
+          sw[j][2 * i + 1] = cw[j][2 * i] * ss[i];
+          cw[j][2 * i] *= cc[i];
+          cw[j][2 * i + 1] *= cc[i];
         }
       }
     }
   }
-  const int src = sub * LPR + pl;
-  const int64_t xoff = b * a.xsb[t] + n * a.xsn[t] + e0, yoff = b * a.ysb[t] + n * a.ysn[t] + e0;
 
-  for (int hb = h0; hb < h1; hb += RPW * kRowsInFlight) {
-    Raw8<DT> raw[kRowsInFlight];
 #pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const int h = hb + u * RPW + sub;
-      if (live && h < h1) raw[u].load(a.x[t], xoff + h * a.xsh[t]);
-      else raw[u].zero();
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * RPW + sub;
+    float v[CH][8];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) raw[u][j].values(v[j]);
+    float r = 1.f;
+    if (a.norm) {
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) tc::fma2(s0, s1, v[j][i], v[j][i + 1], v[j][i], v[j][i + 1]);
+      s0 += s1;
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      r = rsqrtf(fmaf(s0, a.inv_d, a.eps));
     }
 #pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const int h = hb + u * RPW + sub;
-      float v[8];
-      raw[u].values(v);
-      float r = 1.f;
-      if (a.norm) {
-        float ss = 0.f;
+    for (int j = 0; j < CH; ++j) {
+      float out[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
-      }
-      float p[8], out[8];
-      if constexpr (HALF) {
-        raw[u].from_lane(src).values(p);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = v[i ^ 1];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 8; i += 2) {
+        out[i] = v[j][i];
+        out[i + 1] = v[j][i + 1];
+        tc::mul2(out[i], out[i + 1], cw[j][i], cw[j][i + 1]);
         // (the channels past `rot` take no partner: its value may be infinite)
-        const float y = v[i] * cw[i];
-        out[i] = r * (turned ? fmaf(p[i], sw[i], y) : y);
+        if (turned[j]) {
+          const float p0 = HALF ? v[CH - 1 - j][i] : v[j][i + 1], p1 = HALF ? v[CH - 1 - j][i + 1] : v[j][i];
+          tc::fma2(out[i], out[i + 1], p0, p1, sw[j][i], sw[j][i + 1]);
+        }
+        tc::mul2(out[i], out[i + 1], r, r);
       }
-      if (live && h < h1) Raw8<DT>::store(a.y[t], yoff + h * a.ysh[t], out);
+      if (live[j] && h < h1) Raw8<DT>::store(a.y[t], yoff + h * a.ysh[t] + e[j], out);
     }
   }
 }
 
-template <int DT, int LPR>
-cudaError_t launch_layout(const RopeArgs& a, bool half, cudaStream_t st) {
+// Lanes of a row when each has `chunks` chunks.
+int lanes_per_row(int D, int chunks) { return (D <= 64 ? 8 : D <= 128 ? 16 : 32) / chunks; }
+
+template <int DT, int LPR, bool HALF>
+cudaError_t launch_rows(RopeArgs a, cudaStream_t st) {
+  a.chunk_heads = 32 / LPR * kRowsInFlight<HALF>;
+  a.chunks_q = (a.heads[0] + a.chunk_heads - 1) / a.chunk_heads;
+  a.chunks = a.chunks_q + (a.heads[1] + a.chunk_heads - 1) / a.chunk_heads;
+  const int64_t items = static_cast<int64_t>(a.B) * a.N * a.chunks;
+  if (items >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
+  a.items = static_cast<uint32_t>(items);
   const unsigned ctas = (a.items + kWarpsPerCta - 1) / kWarpsPerCta;
-  if (half) qk_norm_rope_kernel<DT, LPR, true><<<ctas, kWarpsPerCta * 32, 0, st>>>(a);
-  else qk_norm_rope_kernel<DT, LPR, false><<<ctas, kWarpsPerCta * 32, 0, st>>>(a);
+  qk_norm_rope_kernel<DT, LPR, HALF><<<ctas, kWarpsPerCta * 32, 0, st>>>(a);
   return cudaGetLastError();
 }
 
-int lanes_per_row(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
-
 template <int DT>
 cudaError_t launch_dtype(const RopeArgs& a, bool half, cudaStream_t st) {
-  switch (lanes_per_row(a.D)) {
-    case 8: return launch_layout<DT, 8>(a, half, st);
-    case 16: return launch_layout<DT, 16>(a, half, st);
-    default: return launch_layout<DT, 32>(a, half, st);
+  switch (lanes_per_row(a.D, half ? 2 : 1)) {
+    case 4: return launch_rows<DT, 4, true>(a, st);
+    case 8: return half ? launch_rows<DT, 8, true>(a, st) : launch_rows<DT, 8, false>(a, st);
+    case 16: return half ? launch_rows<DT, 16, true>(a, st) : launch_rows<DT, 16, false>(a, st);
+    default: return launch_rows<DT, 32, false>(a, st);
   }
 }
 
@@ -294,12 +306,8 @@ extern "C" VCATTN_API int vcattn_qk_norm_rope(const vcattn_bhnd* q, const vcattn
   a.norm = (flags & VCATTN_ROPE_NORM) ? 1 : 0;
   const int t0 = Hq > 0 ? 0 : 1;
   a.token_major = a.xsh[t0] <= a.xsn[t0];
-  a.chunk_heads = 32 / lanes_per_row(D) * kRowsInFlight;
-  a.chunks_q = (Hq + a.chunk_heads - 1) / a.chunk_heads;
-  a.chunks = a.chunks_q + (Hk + a.chunk_heads - 1) / a.chunk_heads;
-  const int64_t items = static_cast<int64_t>(B) * N * a.chunks;
-  if (items >= (int64_t{1} << 31)) return arg_error("more than 2^31 groups of rows");
-  a.items = static_cast<uint32_t>(items);
+  // (a warp takes four heads or more, so this bounds its count of groups)
+  if (static_cast<int64_t>(B) * N >= (int64_t{1} << 31) / (Hq + Hk)) return arg_error("2^31 head rows or more");
   const bool half = !(flags & VCATTN_ROPE_INTERLEAVED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == VCATTN_DTYPE_BF16  ? launch_dtype<VCATTN_DTYPE_BF16>(a, half, st)

@@ -4,8 +4,8 @@
 // Blocks are 1 x 128 (activations: one scale per row) or 128 x 128 (weights).
 // A NaN in a block makes its scale, and so the whole block, NaN.
 //
-// Sixteen lanes hold one 128-column row segment, eight columns each, in
-// registers as loaded: the maximum is taken on the 16-bit pairs.  Both
+// A few lanes hold one 128-column row segment in registers as loaded: the
+// maximum is taken on the 16-bit pairs.  Both
 // quotients are Markstein's correction of a product with the reciprocal (see
 // DivBy), so the scales and codes are those of IEEE divisions; the one of x / s
 // runs on packed fp32 pairs.  Bound by HBM where the instructions allow: the
@@ -161,45 +161,34 @@ __device__ __forceinline__ void store_codes(const QuantArgs& a, int64_t row, int
   }
 }
 
-// 1 x 128 blocks: half a warp per block, kSegs blocks per half-warp in flight.
-constexpr int kSegs = 4;
+// 1 x 128 blocks: LANES lanes per block, each with every LANES-th chunk of
+// eight columns, so that the block's scale and its reciprocal are computed by
+// few lanes for many elements each.
+constexpr int kLanes = 4;
+constexpr int kChunks = 16 / kLanes;
 
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) quant_rows_blocks_kernel(const QuantArgs a) {
-  const int l = threadIdx.x & 15;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4)) * kSegs;
-  Cols8<DT> v[kSegs];
-  int64_t row[kSegs];
-  int blk[kSegs];
-  {
-    // (a 64-bit division takes longer than the rest of the block)
-    int64_t r;
-    if (a.segs < (int64_t{1} << 31)) r = static_cast<uint32_t>(first) / static_cast<uint32_t>(a.kb);
-    else r = first / a.kb;
-    int b = static_cast<int>(first - r * a.kb);
+  const int l = threadIdx.x % kLanes;
+  const int64_t seg = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
+  // (a 64-bit division takes longer than the rest of the block)
+  int64_t row;
+  if (a.segs < (int64_t{1} << 31)) row = static_cast<uint32_t>(seg) / static_cast<uint32_t>(a.kb);
+  else row = seg / a.kb;
+  const int blk = static_cast<int>(seg - row * a.kb);
+  Cols8<DT> v[kChunks];
 #pragma unroll
-    for (int u = 0; u < kSegs; ++u) {
-      row[u] = r;
-      blk[u] = b;
-      if (++b == a.kb) {
-        b = 0;
-        ++r;
-      }
-    }
-  }
+  for (int u = 0; u < kChunks; ++u) load_cols<DT, VEC>(a, seg < a.segs, row, blk * kBlk + (u * kLanes + l) * 8, v[u]);
+  float m = v[0].max_abs();
 #pragma unroll
-  for (int u = 0; u < kSegs; ++u) load_cols<DT, VEC>(a, first + u < a.segs, row[u], blk[u] * kBlk + l * 8, v[u]);
+  for (int u = 1; u < kChunks; ++u) m = max_nan(m, v[u].max_abs());
 #pragma unroll
-  for (int u = 0; u < kSegs; ++u) {
-    float m = v[u].max_abs();
+  for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (seg >= a.segs) return;
+  const float s = block_scale(m), y = __frcp_rn(s);
+  if (l == 0) a.scale[row * a.ssm + blk * a.ssk] = s;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (first + u < a.segs) {
-      const float s = block_scale(m);
-      if (l == 0) a.scale[row[u] * a.ssm + blk[u] * a.ssk] = s;
-      store_codes<DT>(a, row[u], blk[u] * kBlk + l * 8, v[u], s, __frcp_rn(s));
-    }
-  }
+  for (int u = 0; u < kChunks; ++u) store_codes<DT>(a, row, blk * kBlk + (u * kLanes + l) * 8, v[u], s, y);
 }
 
 // 128 x 128 blocks: one CTA per block, eight rows of eight columns per thread.
@@ -232,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) quant_square_blocks_kernel(const Qua
 template <int DT, bool VEC>
 cudaError_t launch(const QuantArgs& a, int rows, cudaStream_t st) {
   if (rows == 1) {
-    const int64_t per = (kThreads / 16) * kSegs;
+    const int64_t per = kThreads / kLanes;
     quant_rows_blocks_kernel<DT, VEC><<<static_cast<unsigned>((a.segs + per - 1) / per), kThreads, 0, st>>>(a);
   } else {
     const int64_t n = (a.M + kBlk - 1) / kBlk * a.kb;
