@@ -289,6 +289,7 @@ template <int D> constexpr int kSmem = 4 * kTile<D>;   // K and V, two stages
 template <int DT, int D>
 __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
+  grid_release();
   const PackedTile t = a.tiles[blockIdx.x];
   const int kvh = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -315,6 +316,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedAr
   }
   rows.finish_sum();
   rows.store(a, t, (static_cast<int64_t>(t.slot) * a.Hk + kvh) * kPackedRows + warp * 16);
+  grid_wait();
 }
 
 // ---- 16 rows: the warps take every fourth tile of sixteen keys ---------------
@@ -330,6 +332,7 @@ template <int D> constexpr int kFewSmem = kWarps * kFewStages * 2 * kFewTile<D>;
 template <int DT, int D>
 __global__ void __launch_bounds__(kWarps * 32, 2) attn_packed_few_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
+  grid_release();
   const PackedTile t = a.tiles[blockIdx.x];
   const int kvh = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -387,7 +390,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_packed_few_kernel(const P
   constexpr int C = D / 32;   // channels per lane: lane = row * 2 + half
   const int row = lane >> 1, c0 = warp * (D / 4) + (lane & 1) * (D / 8);
   const int r = t.r0 + row, tok = r / a.G;
-  if (r >= t.lq * a.G || t.q0 + tok >= a.Tq) return;
+  if (r >= t.lq * a.G || t.q0 + tok >= a.Tq) {
+    grid_wait();
+    return;
+  }
   float m = -INFINITY, l = 0.f, acc[D / 8];
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) m = fmaxf(m, wm[w][row]);
@@ -415,6 +421,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_packed_few_kernel(const P
 #pragma unroll
     for (int c = 0; c < D / 8; c += 2) *reinterpret_cast<uint32_t*>(p + c) = pack2<DT>(acc[c] * inv, acc[c + 1] * inv);
   }
+  grid_wait();
+}
+
+// A kernel that may start while the one before it in the stream still runs
+// (programmatic dependent launch; `after`: that one is of this call).  The
+// kernels release the next one at their start, wait for the one before where
+// they need its results, and otherwise at their end, so that a kernel's
+// completion implies that of all before it.
+template <typename K, typename... A>
+cudaError_t launch_after(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool after, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, one warp per row.  The
@@ -422,26 +449,52 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_packed_few_kernel(const P
 // query head head * G + g.
 template <int DT, int D, int R>
 __global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs a, int heads, int G) {
+  grid_wait();   // the parts
   const PackedJoin jn = a.joins[blockIdx.x / (R / 8)];
   const int row = (blockIdx.x % (R / 8)) * 8 + (threadIdx.x >> 5), head = blockIdx.y, lane = threadIdx.x & 31;
   const int r = jn.r0 + row, tok = r / G;
   if (tok >= jn.lq || jn.q0 + tok >= a.Tq) return;
   const int64_t step = static_cast<int64_t>(heads) * R;
   const int64_t first = (static_cast<int64_t>(jn.slot0) * heads + head) * R + row;
-  float mx = -INFINITY;
+  constexpr int C = D / 32, P = 8;   // channels of a lane, parts in flight
+  float acc[C], den = 0.f, mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.f;
   for (int p = lane; p < jn.pieces; p += 32) mx = fmaxf(mx, a.part_ml[(first + p * step) * 2]);
   mx = warp_max(mx);
   const float base = mx == -INFINITY ? 0.f : mx;
-  constexpr int C = D / 32;
-  float acc[C], den = 0.f;
+  for (int p0 = 0; p0 < jn.pieces; p0 += 32) {
+    // lane p holds the weight and the sum of part p0 + p
+    float w = 0.f, l = 0.f;
+    if (p0 + lane < jn.pieces) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (first + (p0 + lane) * step) * 2);
+      w = exp2f(ml.x - base);
+      l = ml.y;
+    }
+    const int n = min(32, jn.pieces - p0);
+    for (int q = 0; q < n; q += P) {
+      float x[P][C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  for (int p = 0; p < jn.pieces; ++p) {
-    const int64_t i = first + p * step;
-    const float w = exp2f(a.part_ml[i * 2] - base);
-    den = fmaf(w, a.part_ml[i * 2 + 1], den);
+      for (int u = 0; u < P; ++u) {
+        const float* src = a.part_o + (first + (p0 + min(q + u, n - 1)) * step) * D + lane * C;
+        if constexpr (C == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src);
+          x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
+        } else {
+          const float2 f = *reinterpret_cast<const float2*>(src);
+          x[u][0] = f.x; x[u][1] = f.y;
+        }
+      }
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = fmaf(w, a.part_o[i * D + lane * C + c], acc[c]);
+      for (int u = 0; u < P; ++u) {   // (in the order of the parts)
+        const float wu = __shfl_sync(0xffffffffu, w, (q + u) & 31), lu = __shfl_sync(0xffffffffu, l, (q + u) & 31);
+        if (q + u < n) {
+          den = fmaf(wu, lu, den);
+#pragma unroll
+          for (int c = 0; c < C; ++c) acc[c] = fmaf(wu, x[u][c], acc[c]);
+        }
+      }
+    }
   }
   const float inv = den != 0.f ? __fdiv_rn(1.f, den) : 0.f;
   uint16_t* o = static_cast<uint16_t*>(a.out) + (head * G + r - tok * G) * a.osh + static_cast<int64_t>(jn.q0 + tok) * a.osn;
@@ -452,35 +505,35 @@ __global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs 
 template <int DT, int D, int R>
 cudaError_t join(const PackedArgs& a, int heads, int G, cudaStream_t st) {
   if (a.n_joins == 0) return cudaSuccess;
-  attn_packed_join_kernel<DT, D, R><<<dim3(a.n_joins * (R / 8), heads), 256, 0, st>>>(a, heads, G);
-  return cudaGetLastError();
+  return launch_after(attn_packed_join_kernel<DT, D, R>, dim3(a.n_joins * (R / 8), heads), 256, 0, st, true, a, heads, G);
 }
 
-// The three lists of a batch (kPackedFewRows, kPackedRows, kPackedWideRows rows per tile).
+// The three lists of a batch (kPackedFewRows, kPackedRows, kPackedWideRows
+// rows per tile).  The lists do not depend on each other, so the CTAs of the
+// next one start on the SMs that the one before no longer fills.
 template <int DT, int D>
 cudaError_t launch(const PackedArgs (&list)[3], cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   const PackedArgs &few = list[0], &mid = list[1], &wide = list[2];
+  bool after = false;
   if (wide.n_tiles > 0) {
     e = launch_attn_packed_tc(wide, DT, st);
-    if (e == cudaSuccess) e = join<DT, D, kPackedWideRows>(wide, wide.Hq, 1, st);
+    after = true;
   }
   if (e == cudaSuccess && mid.n_tiles > 0) {
     auto k = attn_packed_kernel<DT, D>;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<D>);
-    if (e != cudaSuccess) return e;
-    k<<<dim3(mid.n_tiles, mid.Hk), kWarps * 32, kSmem<D>, st>>>(mid);
-    e = cudaGetLastError();
-    if (e == cudaSuccess) e = join<DT, D, kPackedRows>(mid, mid.Hk, mid.G, st);
+    if (e == cudaSuccess) e = launch_after(k, dim3(mid.n_tiles, mid.Hk), kWarps * 32, kSmem<D>, st, after, mid);
+    after = true;
   }
   if (e == cudaSuccess && few.n_tiles > 0) {
     auto k = attn_packed_few_kernel<DT, D>;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<D>);
-    if (e != cudaSuccess) return e;
-    k<<<dim3(few.n_tiles, few.Hk), kWarps * 32, kFewSmem<D>, st>>>(few);
-    e = cudaGetLastError();
-    if (e == cudaSuccess) e = join<DT, D, kPackedFewRows>(few, few.Hk, few.G, st);
+    if (e == cudaSuccess) e = launch_after(k, dim3(few.n_tiles, few.Hk), kWarps * 32, kFewSmem<D>, st, after, few);
   }
+  if (e == cudaSuccess) e = join<DT, D, kPackedWideRows>(wide, wide.Hq, 1, st);
+  if (e == cudaSuccess) e = join<DT, D, kPackedRows>(mid, mid.Hk, mid.G, st);
+  if (e == cudaSuccess) e = join<DT, D, kPackedFewRows>(few, few.Hk, few.G, st);
   return e;
 }
 

@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   DevStatus* status = &g_attn_packed_status;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int head = blockIdx.x % a.Hq;
+  grid_release();
   if (tid == 0) {
     sm.t = a.tiles[blockIdx.x / a.Hq];
     sm.abort = 0;
