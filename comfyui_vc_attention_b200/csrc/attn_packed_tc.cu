@@ -14,8 +14,8 @@
 // TMEM columns: S of the halves [0,128) [128,256), O [256,384) [384,512); P
 // (16 bits) goes over the first 64 columns of its own S and feeds the P V
 // product from tensor memory.  MMAs complete in issue order, so per half the
-// issuer runs  P V (tile j), S (tile j + 1)  as soon as P of tile j is
-// there, and while the softmax of one half works the tensor pipe runs the
+// issuer runs  P V (tile j), S (tile j + 1)  as P of tile j comes in
+// (two parts of 64 keys), and while the softmax of one half works the tensor pipe runs the
 // other half's two products.  When S of tile j is complete, so is the P V
 // product of tile j - 1: the softmax thread may rescale its row of O without a
 // hand-off.  It does so only when the row's maximum outgrows m by more than 8
@@ -65,7 +65,7 @@ template <int D> struct PackedSmem {
   alignas(8) uint64_t empty[Cfg<D>::kStages];
   alignas(8) uint64_t v_ok[Cfg<D>::kStages / 2];   // the V tile of a stage may be used
   alignas(8) uint64_t s_full[2];
-  alignas(8) uint64_t p_full[2];
+  alignas(8) uint64_t p_full[2][2];                // P of the first and the last 64 keys
   alignas(8) uint64_t o_full[2];
   alignas(8) uint64_t drain;
   uint32_t tmem_base;
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kStages / 2; ++s) mbar_init(&sm.v_ok[s], 2);
     for (int h = 0; h < 2; ++h) {
       mbar_init(&sm.s_full[h], 1);
-      mbar_init(&sm.p_full[h], 4);
+      mbar_init(&sm.p_full[h][0], 4);
+      mbar_init(&sm.p_full[h][1], 4);
       mbar_init(&sm.o_full[h], 1);
     }
     mbar_init(&sm.drain, 1);
@@ -234,12 +235,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_commit_if(&sm.s_full[h], leader);
       };
-      auto issue_pv = [&](int h, int stage, bool first) {
+      auto issue_pv = [&](int h, int stage, int j) {
         const uint32_t va = smem_u32(sm.kv[stage]);
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)   // 16 keys = two groups of eight 128-byte rows
-          mma_f16_ts_if(tbase + kColO + h * 128, tbase + kColS + h * 128 + kk * 8,
-                        smem_desc(va + kk * 2048, C::kBlockBytes, 1024), id_pv, !(first && kk == 0), leader);
+        for (int part = 0; part < 2; ++part) {
+          if (!mbar_wait(&sm.p_full[h][part], j & 1, abort, status, 6)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4 * part; kk < 4 * part + 4; ++kk)   // 16 keys = two groups of eight 128-byte rows
+            mma_f16_ts_if(tbase + kColO + h * 128, tbase + kColS + h * 128 + kk * 8,
+                          smem_desc(va + kk * 2048, C::kBlockBytes, 1024), id_pv, j > 0 || kk > 0, leader);
+        }
+        return true;
       };
       bool ok = n > 0 && mbar_wait(&sm.q_full, 0, abort, status, 2) && mbar_wait(&sm.full[0], 0, abort, status, 3);
       if (ok) {
@@ -257,9 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = 0; h < 2; ++h) {
           const int nh = h ? n1 : n0;
           if (ok && j < nh) {
-            if (!(ok = mbar_wait(&sm.p_full[h], j & 1, abort, status, 6))) break;
-            tc_fence_after();
-            issue_pv(h, sv, j == 0);
+            if (!(ok = issue_pv(h, sv, j))) break;
             if (j + 1 < nh) issue_s(h, sk);
             else tc_commit_if(&sm.o_full[h], leader);
           }
@@ -385,10 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           w[e] = pack16<DT>(p0, p1);
         }
         tmem_st16(ts + 16 * c, w);
+        if (c % 2 == 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          warp_arrive(&sm.p_full[h][c / 2], lane);
+        }
       }
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&sm.p_full[h], lane);
     }
     if (ok && nh > 0) ok = mbar_wait(&sm.o_full[h], 0, abort, status, 9);
     tc_fence_after();

@@ -3,7 +3,7 @@
 // with kb running over blocks of 128 columns (the last one may be short).
 //
 // tcgen05 kind::f8f6f4: each k-block of 128 is one accumulation of four MMAs in
-// tensor memory, in one of two buffers; the promotion warps read the finished
+// tensor memory, in one of two or four buffers; the promotion warps read the finished
 // block sum and add it to fp32 registers with its scale while the next block
 // runs.  Thread = output row (TMEM lane) and 64 columns, so the scale of a
 // block is one scalar per thread.
@@ -84,7 +84,7 @@ template <int BN> struct MmCfg {
   static constexpr int kStages = BN == 256 ? 3 : 5;
   static constexpr int kPromo = BN / 64 * 4;               // promotion warps
   static constexpr int kThreads = 128 + 32 * kPromo;
-  static constexpr int kTmemCols = 2 * BN;
+  static constexpr int kBufs = 512 / BN;                   // block sums in tensor memory
   // Output staging of a warp: 32 bytes of each of its 32 rows at a time, 16
   // bytes apart so that the rows start in different banks.
   static constexpr int kOutPitch = 128 + 16;
@@ -99,8 +99,8 @@ template <int BN> struct MmSmem {
   alignas(16) float scale[2][BN / 128][kBM][kGroup];
   alignas(8) uint64_t full[MmCfg<BN>::kStages];
   alignas(8) uint64_t empty[MmCfg<BN>::kStages];
-  alignas(8) uint64_t t_full[2];
-  alignas(8) uint64_t t_empty[2];
+  alignas(8) uint64_t t_full[MmCfg<BN>::kBufs];
+  alignas(8) uint64_t t_empty[MmCfg<BN>::kBufs];
   alignas(8) uint64_t s_full[2];
   alignas(8) uint64_t s_empty[2];
   alignas(8) uint64_t drain;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     matmul_blocks_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const MatmulArgs a) {
   using Cfg = MmCfg<BN>;
-  constexpr int kStages = Cfg::kStages;
+  constexpr int kStages = Cfg::kStages, kBufs = Cfg::kBufs;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   MmSmem<BN>& sm = *reinterpret_cast<MmSmem<BN>*>(smem_raw + pad);
@@ -135,9 +135,11 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < Cfg::kBufs; ++b) {
       mbar_init(&sm.t_full[b], 1);
       mbar_init(&sm.t_empty[b], Cfg::kPromo);
+    }
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.s_full[b], 2);
       mbar_init(&sm.s_empty[b], Cfg::kPromo);
     }
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&sm.tmem_base, Cfg::kTmemCols);
+    tmem_alloc(&sm.tmem_base, 512);
     tmem_relinquish();
   }
   __syncthreads();
@@ -196,8 +198,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     bool ok = true;
     for (int t = t0; ok && t < a.tiles; t += t_step) {
       for (int k = kb0; k < kb1; ++k, ++it) {
-        const int s = it % kStages, b = it & 1;
-        if (it >= 2 && !(ok = mbar_wait(&sm.t_empty[b], ((it >> 1) + 1) & 1, abort, status, 2))) break;
+        const int s = it % kStages, b = it % kBufs;
+        if (it >= kBufs && !(ok = mbar_wait(&sm.t_empty[b], ((it / kBufs) + 1) & 1, abort, status, 2))) break;
         if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, abort, status, 3))) break;
         tc_fence_after();
         const uint32_t aa = smem_u32(sm.a[s]), ba = smem_u32(sm.b[s]);
@@ -294,8 +296,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 32; c += 2) fma2(acc[h * 32 + c], acc[h * 32 + c + 1], x[c], x[c + 1], s[u], s[u]);
           }
-          b ^= 1;
-          b_par ^= b ^ 1;
+          b = (b + 1) % kBufs;
+          b_par ^= b == 0;
         }
       }
       if (!ok || *abort) continue;
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     }
   }
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tbase, Cfg::kTmemCols);
+  if (warp == 1) tmem_dealloc(tbase, 512);
   if constexpr (SPLIT) {
     // every rank adds the parts of its share of the rows, in rank order
     __syncwarp();
