@@ -290,8 +290,8 @@ template <int DT, int D>
 __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   grid_release();
-  const PackedTile t = a.tiles[blockIdx.x];
-  const int kvh = blockIdx.y;
+  const PackedTile t = a.tiles[blockIdx.x / a.Hk];   // longest first, over all heads
+  const int kvh = blockIdx.x % a.Hk;
   const int tid = threadIdx.x, warp = tid >> 5;
   const uint32_t s0 = smem_addr(smem);
   Rows16<DT, D> rows;
@@ -322,43 +322,46 @@ __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedAr
 // ---- 16 rows: the warps take every fourth tile of sixteen keys ---------------
 // A single new token gives a KV head's group only a few rows: the work is to
 // stream K and V once.  Each warp fills and reads its own ring (no barrier
-// until the end), two CTAs per SM keep about 128 KB in flight, and the four
-// partial results are added in warp order through shared memory.
+// until the end), and the four partial results are added in warp order through
+// shared memory.  Two rings: three stages with two CTAs per SM keep 128 KB in
+// flight (64 sequences of 2048 keys, 8 KV heads of 128: 91 us, 5.9 TB/s; two
+// stages with three CTAs: 118 us); two stages let three CTAs start at once,
+// which is better when no CTA has to wait for that (12 sequences of 1 to 8192
+// keys, 344 CTAs: 38 against 50 us).
 constexpr int kFewKeys = 16;
-constexpr int kFewStages = 3;
 template <int D> constexpr int kFewTile = kFewKeys * kPitch<D>;
-template <int D> constexpr int kFewSmem = kWarps * kFewStages * 2 * kFewTile<D>;
+template <int D, int STAGES> constexpr int kFewSmem = kWarps * STAGES * 2 * kFewTile<D>;
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kWarps * 32, 2) attn_packed_few_kernel(const PackedArgs a) {
+template <int DT, int D, int STAGES>
+__global__ void __launch_bounds__(kWarps * 32, STAGES == 2 ? 3 : 2) attn_packed_few_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   grid_release();
-  const PackedTile t = a.tiles[blockIdx.x];
-  const int kvh = blockIdx.y;
+  const PackedTile t = a.tiles[blockIdx.x / a.Hk];   // longest first, over all heads
+  const int kvh = blockIdx.x % a.Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * kFewStages * 2 * kFewTile<D>;
+  uint8_t* ring = smem + warp * STAGES * 2 * kFewTile<D>;
   const uint32_t r0 = smem_addr(ring);
   const int tiles = t.ke > t.kb ? (t.ke - t.kb + kFewKeys - 1) / kFewKeys : 0;
   const int steps = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
   auto load = [&](int j) {
-    const uint32_t dst = r0 + (j % kFewStages) * 2 * kFewTile<D>;
+    const uint32_t dst = r0 + (j % STAGES) * 2 * kFewTile<D>;
     const int key0 = t.kb + (j * kWarps + warp) * kFewKeys;
     load_keys<D, kFewKeys, 32>(dst, a, a.k, a.ksh, a.ksn, t, kvh, key0, lane);
     load_keys<D, kFewKeys, 32>(dst + kFewTile<D>, a, a.v, a.vsh, a.vsn, t, kvh, key0, lane);
   };
 #pragma unroll
-  for (int j = 0; j < kFewStages - 1; ++j) {
+  for (int j = 0; j < STAGES - 1; ++j) {
     if (j < steps) load(j);
     copy_commit();
   }
   Rows16<DT, D> rows;
   rows.start(a, t, kvh, t.r0, lane);
   for (int j = 0; j < steps; ++j) {
-    copy_wait<kFewStages - 2>();
+    copy_wait<STAGES - 2>();
     __syncwarp();
-    if (j + kFewStages - 1 < steps) load(j + kFewStages - 1);   // (over the tile that every lane has finished with)
+    if (j + STAGES - 1 < steps) load(j + STAGES - 1);   // (over the tile that every lane has finished with)
     copy_commit();
-    const int st = (j % kFewStages) * 2 * kFewTile<D>;
+    const int st = (j % STAGES) * 2 * kFewTile<D>;
     rows.template step<kFewKeys>(a, r0 + st, r0 + st + kFewTile<D>, ring + st + kFewTile<D>,
                                  t.kb + (j * kWarps + warp) * kFewKeys);
   }
@@ -508,6 +511,21 @@ cudaError_t join(const PackedArgs& a, int heads, int G, cudaStream_t st) {
   return launch_after(attn_packed_join_kernel<DT, D, R>, dim3(a.n_joins * (R / 8), heads), 256, 0, st, true, a, heads, G);
 }
 
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n > 0 ? n : 148;
+}
+
+template <int DT, int D, int STAGES>
+cudaError_t launch_few(const PackedArgs& a, unsigned ctas, bool after, cudaStream_t st) {
+  auto k = attn_packed_few_kernel<DT, D, STAGES>;
+  constexpr int smem = kFewSmem<D, STAGES>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e == cudaSuccess ? launch_after(k, dim3(ctas), kWarps * 32, smem, st, after, a) : e;
+}
+
 // The three lists of a batch (kPackedFewRows, kPackedRows, kPackedWideRows
 // rows per tile).  The lists do not depend on each other, so the CTAs of the
 // next one start on the SMs that the one before no longer fills.
@@ -523,13 +541,12 @@ cudaError_t launch(const PackedArgs (&list)[3], cudaStream_t st) {
   if (e == cudaSuccess && mid.n_tiles > 0) {
     auto k = attn_packed_kernel<DT, D>;
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem<D>);
-    if (e == cudaSuccess) e = launch_after(k, dim3(mid.n_tiles, mid.Hk), kWarps * 32, kSmem<D>, st, after, mid);
+    if (e == cudaSuccess) e = launch_after(k, dim3(static_cast<unsigned>(mid.n_tiles) * mid.Hk), kWarps * 32, kSmem<D>, st, after, mid);
     after = true;
   }
   if (e == cudaSuccess && few.n_tiles > 0) {
-    auto k = attn_packed_few_kernel<DT, D>;
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem<D>);
-    if (e == cudaSuccess) e = launch_after(k, dim3(few.n_tiles, few.Hk), kWarps * 32, kFewSmem<D>, st, after, few);
+    const unsigned ctas = static_cast<unsigned>(few.n_tiles) * few.Hk;
+    e = ctas <= 3u * sm_count() ? launch_few<DT, D, 2>(few, ctas, after, st) : launch_few<DT, D, 3>(few, ctas, after, st);
   }
   if (e == cudaSuccess) e = join<DT, D, kPackedWideRows>(wide, wide.Hq, 1, st);
   if (e == cudaSuccess) e = join<DT, D, kPackedRows>(mid, mid.Hk, mid.G, st);

@@ -13,8 +13,9 @@ register MMAs over the rows of a KV head's group for few).  Forward only.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -26,12 +27,23 @@ __all__ = ["PackedPlan", "packed_plan", "packed_attention"]
 
 SMS = 148
 
-# Rows of a tile, granularity of a key range, the shortest range worth a tile of
-# its own, and the tiles per SM that keep it busy: register-MMA tiles of (token,
-# group head) rows, and tcgen05 tiles of tokens.
-FEW = (16, 64, 256, 4)
-MID = (64, 64, 256, 4)
-WIDE = (256, 128, 1024, 1)
+
+class _Shape(NamedTuple):
+    """One of the three kinds of tiles: rows per tile, granularity of a key
+    range, CTAs resident on the SMs, and what a tile, a part of a split tile
+    and a join cost beside their keys, in keys (for the choice of a split)."""
+    rows: int
+    step: int
+    slots: int
+    tile_cost: int
+    part_cost: int
+    join_cost: int
+
+
+# Register-MMA tiles of (token, group head) rows, and tcgen05 tiles of tokens.
+FEW = _Shape(16, 64, 2 * SMS, 0, 0, 0)
+MID = _Shape(64, 64, 3 * SMS, 128, 100, 160)
+WIDE = _Shape(256, 128, SMS, 320, 450, 640)
 WIDE_FROM = 64   # queries of a sequence that goes to the tcgen05 kernel
 
 
@@ -63,23 +75,56 @@ def _lengths(x, what) -> np.ndarray:
     return a
 
 
-def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
+def _pieces(ke: np.ndarray, heads: int, shape: _Shape):
+    """Key ranges per tile and their length, for tiles of ``ke`` keys on each of
+    ``heads`` heads."""
+    def spans(share):
+        n = np.maximum(1, -(-ke // share))
+        span = np.maximum(shape.step, -(-(-(-ke // n)) // shape.step) * shape.step)
+        return np.maximum(1, -(-ke // span)), span
+
+    total, longest = int(ke.sum()) * heads, max(1, int(ke.max(initial=0)))
+    if shape is FEW:
+        # Bound by the K/V bytes, which one CTA per SM nearly draws: tiles are
+        # split only where one holds more than an SM's share (12 sequences of 1
+        # to 8192 keys: 45 us unsplit at two CTAs' share, 38 us; 64 of 2048:
+        # 91 us whole, 103 in halves).
+        return spans(longest if longest <= total / SMS else max(4 * shape.step, math.ceil(total / shape.slots)))
+    # Bound by the tensor cores: splitting evens out the CTAs and costs partial
+    # results and a join.  Of a few splits, the one whose longest run of CTAs on
+    # a slot is estimated shortest (longest first: no shorter than the longest
+    # tile, the mean, and the two tiles that meet where the slots run out).
+    best = None
+    for c in (0.0, 0.75, 1.0, 1.5, 2.0, 3.0):
+        share = max(4 * shape.step, math.ceil(total / (shape.slots * c))) if c else longest
+        if c and share >= longest:
+            continue
+        n, span = spans(share)
+        size = np.repeat(np.minimum(span, ke) + np.where(n > 1, shape.part_cost, 0) + shape.tile_cost, n)
+        size = np.sort(size)[::-1]
+        cost = max(int(size[0]), int(size.sum()) * heads / shape.slots)
+        at = shape.slots // heads
+        if 0 < at < len(size):
+            cost = max(cost, int(size[at - 1]) + int(size[at]))
+        cost += shape.join_cost if (n > 1).any() else 0
+        if best is None or cost < best[0]:
+            best = (cost, n, span)
+    return best[1], best[2]
+
+
+def _tiles(q0, ql, k0, kl, group, heads, causal, shape: _Shape):
     """Tile and join records (int32 arrays) of the given sequences, and the
-    number of partial results.  A batch that would leave SMs idle splits its
-    longest key ranges."""
-    rows, step, least, per_sm = shape
-    per = -(-(ql * group) // rows)
+    number of partial results."""
+    none = np.zeros((0, 8), dtype=np.int32)
+    if not ql.any():
+        return none, none, 0
+    per = -(-(ql * group) // shape.rows)
     seq = np.repeat(np.arange(len(ql)), per)
-    r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * rows
+    r0 = (np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)) * shape.rows
     lq, lk = ql[seq], kl[seq]
-    last = np.minimum((r0 + rows - 1) // group, lq - 1)
-    ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk.copy()
-    pieces = np.ones(len(seq), dtype=np.int64)
-    work = int(ke.sum()) * heads
-    if len(seq) * heads < per_sm * SMS and work:
-        pieces = np.maximum(1, -(-ke // max(least, -(-work // (per_sm * SMS)))))
-    span = -(-(-(-ke // pieces)) // step) * step             # keys per piece
-    pieces = np.maximum(1, -(-ke // np.maximum(span, 1)))
+    last = np.minimum((r0 + shape.rows - 1) // group, lq - 1)
+    ke = np.clip(last + 1 + lk - lq, 0, lk) if causal else lk
+    pieces, span = _pieces(ke, heads, shape)
     row = np.repeat(np.arange(len(seq)), pieces)
     piece = np.arange(len(row)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
     kb = piece * span[row]
@@ -87,8 +132,10 @@ def _tiles(q0, ql, k0, kl, group, heads, causal, shape):
     slot = np.where(split, np.cumsum(split) - 1, -1)
     tiles = np.stack([q0[seq][row], lq[row], k0[seq][row], lk[row], r0[row], kb,
                       np.minimum(kb + span[row], ke[row]), slot], axis=1).astype(np.int32)
-    tiles = np.ascontiguousarray(tiles[np.argsort(-(tiles[:, 6] - tiles[:, 5]), kind="stable")])   # longest first
+    tiles = tiles[np.argsort(tiles[:, 5] - tiles[:, 6], kind="stable")]   # longest first
     js = np.nonzero(pieces > 1)[0]
+    if not len(js):
+        return tiles, none, 0
     joins = np.zeros((len(js), 8), dtype=np.int32)
     joins[:, 0], joins[:, 1], joins[:, 2] = q0[seq][js], lq[js], r0[js]
     joins[:, 3], joins[:, 4] = np.cumsum(pieces[js]) - pieces[js], pieces[js]
@@ -120,18 +167,17 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
         raise ValueError("a sequence has 2^31 rows or more")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     q0, k0 = np.cumsum(ql) - ql, np.cumsum(kl) - kl
-    wide, few = ql >= WIDE_FROM, ql * g <= FEW[0]
+    wide, few = ql >= WIDE_FROM, ql * g <= FEW.rows
     lists = ((few & ~wide, g, kv_heads, FEW), (~few & ~wide, g, kv_heads, MID), (wide, 1, heads, WIDE))
-    tiles, joins, slots, need = [], [], [], 0
-    for pick, group, hs, shape in lists:
-        t, j, n = _tiles(q0[pick], ql[pick], k0[pick], kl[pick], group, hs, causal, shape)
-        tiles.append(torch.from_numpy(t).to(dev))
-        joins.append(torch.from_numpy(j).to(dev))
-        slots.append(n)
-        need += n * hs * shape[0] * (head_dim + 2) * 4
-    work = N.PackedWork(tuple(t.data_ptr() for t in tiles), tuple(j.data_ptr() for j in joins),
-                        tuple(t.shape[0] for t in tiles), tuple(j.shape[0] for j in joins), tuple(slots))
-    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), tuple(tiles), tuple(joins),
+    made = [_tiles(q0[pick], ql[pick], k0[pick], kl[pick], group, hs, causal, shape)
+            for pick, group, hs, shape in lists]
+    need = sum(m[2] * hs * shape.rows * (head_dim + 2) * 4 for m, (_, _, hs, shape) in zip(made, lists))
+    # one upload for all records
+    host = np.concatenate([m[i] for i in (0, 1) for m in made])
+    recs = torch.from_numpy(host).to(dev).split([len(m[i]) for i in (0, 1) for m in made])
+    work = N.PackedWork(tuple(r.data_ptr() for r in recs[:3]), tuple(r.data_ptr() for r in recs[3:]),
+                        tuple(len(r) for r in recs[:3]), tuple(len(r) for r in recs[3:]), tuple(m[2] for m in made))
+    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), recs[:3], recs[3:],
                       work, need)
 
 
