@@ -54,14 +54,11 @@ def out_view(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> Tuple[N
     """``out`` checked against its input, or a new buffer in the token layout of
     the input: token-major rows (the ComfyUI (B, N, H*D) path) stay so."""
     if out is None:
-        b, h, n, d = x.shape
-        if x.stride(1) < x.stride(2):
-            out = torch.empty_strided((b, h, n, d), (n * h * d, d, h * d, 1), dtype=x.dtype, device=x.device)
-        else:
-            out = torch.empty((b, h, n, d), dtype=x.dtype, device=x.device)
-        sb, sh, sn, _ = out.stride()
-        if (sb | sh | sn) * x.element_size() & 15:   # rows of an odd length
-            raise ValueError(f"rows of {d} channels of {x.dtype} do not start on 16-byte boundaries")
+        out = torch.empty_like(x)   # (dense, dimensions in x's order)
+        sb, sh, sn, sd = out.stride()
+        if sd != 1:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            sb, sh, sn, _ = out.stride()
         return N.BHND(out.data_ptr(), sb, sh, sn), out
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{what} must match its input: {tuple(x.shape)} {x.dtype} on {x.device}")
