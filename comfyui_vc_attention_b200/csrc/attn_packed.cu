@@ -11,6 +11,7 @@
 // part of the keys writes its unnormalised rows, m and l; the join kernel adds
 // the parts in key order.
 #include "attn_packed.cuh"
+#include "launch.cuh"
 
 #include <string>
 
@@ -427,26 +428,6 @@ __global__ void __launch_bounds__(kWarps * 32, STAGES == 2 ? 3 : 2) attn_packed_
   grid_wait();
 }
 
-// A kernel that may start while the one before it in the stream still runs
-// (programmatic dependent launch; `after`: that one is of this call).  The
-// kernels release the next one at their start, wait for the one before where
-// they need its results, and otherwise at their end, so that a kernel's
-// completion implies that of all before it.
-template <typename K, typename... A>
-cudaError_t launch_after(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool after, const A&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = after ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p, one warp per row.  The
 // parts of a tile of R rows belong to `heads` heads; row = token * G + g is
 // query head head * G + g.
@@ -509,13 +490,6 @@ template <int DT, int D, int R>
 cudaError_t join(const PackedArgs& a, int heads, int G, cudaStream_t st) {
   if (a.n_joins == 0) return cudaSuccess;
   return launch_after(attn_packed_join_kernel<DT, D, R>, dim3(a.n_joins * (R / 8), heads), 256, 0, st, true, a, heads, G);
-}
-
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
 }
 
 template <int DT, int D, int STAGES>

@@ -47,11 +47,6 @@ constexpr int kPackedRows = 64;
 constexpr int kPackedWideRows = 256;
 constexpr int kListRows[3] = {kPackedFewRows, kPackedRows, kPackedWideRows};
 
-// Programmatic dependent launch: let the next kernel of the stream start, and
-// wait until the one before has completed (at once if it was a normal launch).
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
-
 cudaError_t launch_attn_packed_tc(const PackedArgs& a, int dtype, cudaStream_t st);
 
 }  // namespace vcattn

@@ -33,6 +33,7 @@
 #include <cuda.h>
 #include <mutex>
 
+#include "launch.cuh"
 #include "tc_common.cuh"
 #include "tc_math.cuh"
 

@@ -16,6 +16,7 @@
 #include <string>
 
 #include "kernels.cuh"
+#include "launch.cuh"
 #include "tc_common.cuh"
 #include "tc_math.cuh"
 
@@ -28,7 +29,7 @@ namespace {
 using namespace tc;
 
 constexpr int kBM = 128;
-constexpr int kBK = 128;
+constexpr int kBK = 128;   // columns of a k-block
 
 struct MatmulArgs {
   const float *sa, *sb;
@@ -40,6 +41,11 @@ struct MatmulArgs {
   int mt, nt, tiles, group;
   int vec_out;   // rows of `out` start on 16-byte boundaries
   int ranks;     // CTAs of a cluster that share a tile's k-blocks (1: persistent CTAs over whole tiles)
+  // Persistent CTAs: `full` tiles run whole (a multiple of the grid); each of
+  // the others is split in `parts` ranges of k-blocks (1: whole), whose sums go
+  // to `part`.
+  int full, parts;
+  float* part;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -118,7 +124,65 @@ __device__ __forceinline__ void tile_coords(const MatmulArgs& a, int t, int& m, 
   m = g * a.group + (r - n * rows);
 }
 
-template <int BN, int ODT, bool SPLIT>
+// How a tile is shared: not at all, its k-blocks by the CTAs of a cluster, or
+// (the tiles of the last round) in parts that a second kernel joins.
+enum Share { kWhole, kCluster, kParts };
+
+// The pieces of work of a CTA, one after the other: k-blocks [k0, k1) of a
+// tile, and which part of it that is (-1: all of it, or a cluster's share).
+template <Share SHARE> struct Pieces;
+template <> struct Pieces<kWhole> {
+  int t = blockIdx.x;
+  __device__ __forceinline__ explicit Pieces(const MatmulArgs&) {}
+  __device__ __forceinline__ bool any(const MatmulArgs& a) const { return t < a.tiles; }
+  __device__ __forceinline__ void next(const MatmulArgs&) { t += gridDim.x; }
+  __device__ __forceinline__ int tile() const { return t; }
+  __device__ __forceinline__ int k0() const { return 0; }
+  __device__ __forceinline__ int k1(const MatmulArgs& a) const { return a.kb; }
+  __device__ __forceinline__ int part() const { return -1; }
+};
+template <> struct Pieces<kCluster> {
+  int t, b, e;
+  __device__ __forceinline__ explicit Pieces(const MatmulArgs& a) {
+    const int rank = static_cast<int>(cluster_rank());
+    t = blockIdx.x / a.ranks;
+    b = static_cast<int>(static_cast<int64_t>(a.kb) * rank / a.ranks);
+    e = static_cast<int>(static_cast<int64_t>(a.kb) * (rank + 1) / a.ranks);
+  }
+  __device__ __forceinline__ bool any(const MatmulArgs& a) const { return t < a.tiles; }
+  __device__ __forceinline__ void next(const MatmulArgs& a) { t = a.tiles; }
+  __device__ __forceinline__ int tile() const { return t; }
+  __device__ __forceinline__ int k0() const { return b; }
+  __device__ __forceinline__ int k1(const MatmulArgs&) const { return e; }
+  __device__ __forceinline__ int part() const { return -1; }
+};
+template <> struct Pieces<kParts> {
+  int u, t, b, e, p;
+  __device__ __forceinline__ explicit Pieces(const MatmulArgs& a) : u(blockIdx.x) { place(a); }
+  __device__ __forceinline__ void place(const MatmulArgs& a) {
+    t = u;
+    b = 0;
+    e = a.kb;
+    p = -1;
+    if (u >= a.full) {
+      t = a.full + (u - a.full) / a.parts;
+      p = (u - a.full) % a.parts;
+      b = static_cast<int>(static_cast<int64_t>(a.kb) * p / a.parts);
+      e = static_cast<int>(static_cast<int64_t>(a.kb) * (p + 1) / a.parts);
+    }
+  }
+  __device__ __forceinline__ bool any(const MatmulArgs& a) const { return t < a.tiles; }
+  __device__ __forceinline__ void next(const MatmulArgs& a) {
+    u += gridDim.x;
+    place(a);
+  }
+  __device__ __forceinline__ int tile() const { return t; }
+  __device__ __forceinline__ int k0() const { return b; }
+  __device__ __forceinline__ int k1(const MatmulArgs&) const { return e; }
+  __device__ __forceinline__ int part() const { return p; }
+};
+
+template <int BN, int ODT, Share SHARE>
 __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     matmul_blocks_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const MatmulArgs a) {
@@ -154,11 +218,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   tc_fence_after();
   const uint32_t tbase = sm.tmem_base;
   volatile int* abort = &sm.abort;
-  // tiles of this CTA, and the k-blocks that it takes of each
-  const int t0 = SPLIT ? blockIdx.x / a.ranks : blockIdx.x, t_step = SPLIT ? a.tiles : gridDim.x;
-  const int rank = SPLIT ? static_cast<int>(cluster_rank()) : 0;
-  const int kb0 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kb) * rank / a.ranks) : 0;
-  const int kb1 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kb) * (rank + 1) / a.ranks) : a.kb;
+  if constexpr (SHARE == kParts) grid_release();
   if (warp < 4) {
   // BN = 256 is launched at 96 x 640 = 61440 registers: 128 x 56 + 512 x 104 = 60416
   if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n" ::: "memory");
@@ -169,10 +229,10 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       prefetch_tmap(&tm_b);
       int it = 0;
       bool ok = true;
-      for (int t = t0; ok && t < a.tiles; t += t_step) {
+      for (Pieces<SHARE> pc(a); ok && pc.any(a); pc.next(a)) {
         int m, n;
-        tile_coords(a, t, m, n);
-        for (int k = kb0; k < kb1; ++k, ++it) {
+        tile_coords(a, pc.tile(), m, n);
+        for (int k = pc.k0(); k < pc.k1(a); ++k, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !(ok = mbar_wait(&sm.empty[s], ((it / kStages) + 1) & 1, abort, status, 1))) break;
           mbar_expect_tx(&sm.full[s], (kBM + BN) * kBK);
@@ -196,8 +256,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const uint32_t idesc = idesc_e4m3(kBM, BN, false);
     int it = 0;
     bool ok = true;
-    for (int t = t0; ok && t < a.tiles; t += t_step) {
-      for (int k = kb0; k < kb1; ++k, ++it) {
+    for (Pieces<SHARE> pc(a); ok && pc.any(a); pc.next(a)) {
+      for (int k = pc.k0(); k < pc.k1(a); ++k, ++it) {
         const int s = it % kStages, b = it % kBufs;
         if (it >= kBufs && !(ok = mbar_wait(&sm.t_empty[b], ((it / kBufs) + 1) & 1, abort, status, 2))) break;
         if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, abort, status, 3))) break;
@@ -221,9 +281,9 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const int r = tid - 64;   // rows r and r + 64
     int grp = 0;              // groups handed over
     bool ok = true;
-    for (int t = t0; ok && t < a.tiles; t += t_step) {
+    for (Pieces<SHARE> pc(a); ok && pc.any(a); pc.next(a)) {
       int mt, nt;
-      tile_coords(a, t, mt, nt);
+      tile_coords(a, pc.tile(), mt, nt);
       // (rows and columns past the matrix take the scale of the last one: nothing of them is written)
       const float* sa0 = a.sa + static_cast<int64_t>(min(mt * kBM + r, a.M - 1)) * a.sam;
       const float* sa1 = a.sa + static_cast<int64_t>(min(mt * kBM + r + 64, a.M - 1)) * a.sam;
@@ -233,15 +293,15 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       auto load = [&](int k) {
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
-          const int kk = min(k + u, kb1 - 1);
+          const int kk = min(k + u, pc.k1(a) - 1);
           x0[u] = __ldg(sa0 + kk * a.sak);
           x1[u] = __ldg(sa1 + kk * a.sak);
           y0[u] = __ldg(sb + kk * a.sbk);
           if constexpr (BN == 256) y1[u] = __ldg(sb + sb1 + kk * a.sbk);
         }
       };
-      load(kb0);
-      for (int k = kb0; k < kb1; k += kGroup, ++grp) {
+      load(pc.k0());
+      for (int k = pc.k0(); k < pc.k1(a); k += kGroup, ++grp) {
         const int s = grp & 1;
         if (grp >= 2 && !(ok = mbar_wait(&sm.s_empty[s], ((grp >> 1) + 1) & 1, abort, status, 5))) break;
         *reinterpret_cast<float4*>(sm.scale[s][0][r]) = make_float4(x0[0] * y0[0], x0[1] * y0[1], x0[2] * y0[2], x0[3] * y0[3]);
@@ -251,7 +311,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
           *reinterpret_cast<float4*>(sm.scale[s][1][r + 64]) = make_float4(x1[0] * y1[0], x1[1] * y1[1], x1[2] * y1[2], x1[3] * y1[3]);
         }
         warp_arrive(&sm.s_full[s], lane);
-        if (k + kGroup < kb1) load(k + kGroup);   // in flight while the promotion works on this group
+        if (k + kGroup < pc.k1(a)) load(k + kGroup);   // in flight while the promotion works on this group
       }
     }
   }
@@ -265,14 +325,14 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     const float* scale = sm.scale[0][quarter >> 1][wq * 32 + lane];
     uint32_t b = 0, b_par = 0, g = 0, g_par = 0;   // tensor-memory buffer and scale group, and their phases
     bool ok = true;
-    for (int t = t0; ok && t < a.tiles; t += t_step) {
+    for (Pieces<SHARE> pc(a); ok && pc.any(a); pc.next(a)) {
       int mt, nt;
-      tile_coords(a, t, mt, nt);
+      tile_coords(a, pc.tile(), mt, nt);
       const int m0 = mt * kBM + wq * 32, n0 = nt * BN + quarter * 64;
       float acc[64];
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-      for (int k = kb0; ok && k < kb1; k += kGroup) {
+      for (int k = pc.k0(); ok && k < pc.k1(a); k += kGroup) {
         if (!(ok = mbar_wait(&sm.s_full[g], g_par, abort, status, 4))) break;
         const float4 s4 = *reinterpret_cast<const float4*>(scale + g * (BN / 128 * kBM * kGroup));
         warp_arrive(&sm.s_empty[g], lane);
@@ -281,7 +341,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         const float s[kGroup] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
-          if (k + u >= kb1 || !(ok = mbar_wait(&sm.t_full[b], b_par, abort, status, 6))) break;
+          if (k + u >= pc.k1(a) || !(ok = mbar_wait(&sm.t_full[b], b_par, abort, status, 6))) break;
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -301,11 +361,19 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         }
       }
       if (!ok || *abort) continue;
-      if constexpr (SPLIT) {
+      if constexpr (SHARE == kCluster) {
         // this rank's sums over the operand stages (every MMA has read them)
         float* part = reinterpret_cast<float*>(sm.a) + (wq * 32 + lane) * Cfg::kPartPitch + quarter * 64;
 #pragma unroll
         for (int c = 0; c < 64; c += 4) *reinterpret_cast<float4*>(part + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        continue;
+      }
+      if (SHARE == kParts && pc.part() >= 0) {
+        // part of a tile: [tile, part][warp][column / 4][lane], four columns each
+        float4* dst = reinterpret_cast<float4*>(a.part) +
+                      ((static_cast<int64_t>(pc.tile() - a.full) * a.parts + pc.part()) * Cfg::kPromo + (warp - 4)) * 16 * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) dst[c * 32] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         continue;
       }
       // rows through shared memory, so that whole 32-byte sectors go out
@@ -349,12 +417,13 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
   }
   __syncthreads();
   if (warp == 1) tmem_dealloc(tbase, 512);
-  if constexpr (SPLIT) {
+  if constexpr (SHARE == kCluster) {
     // every rank adds the parts of its share of the rows, in rank order
     __syncwarp();
     cluster_sync();
     int mt, nt;
-    tile_coords(a, t0, mt, nt);
+    tile_coords(a, blockIdx.x / a.ranks, mt, nt);
+    const int rank = static_cast<int>(cluster_rank());
     const int rows = *abort ? 0 : min(kBM, a.M - mt * kBM);
     for (int r = rank * (Cfg::kThreads / 32) + warp; r < rows; r += a.ranks * (Cfg::kThreads / 32)) {
       for (int c = lane * 4; c < BN; c += 128) {
@@ -375,6 +444,56 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
     }
     __syncwarp();
     cluster_sync();   // no CTA leaves while another reads its part
+  }
+}
+
+// Adds the parts of the split tiles (128 x 256) in k order: one CTA per 32 rows
+// and 64 columns.
+template <int ODT>
+__global__ void __launch_bounds__(128) matmul_blocks_join_kernel(const MatmulArgs a) {
+  grid_wait();   // the parts
+  constexpr int kPromo = MmCfg<256>::kPromo, ES = ODT == VCATTN_DTYPE_F32 ? 4 : 2;
+  __shared__ float rows[32][64 + 4];
+  const int tile = blockIdx.x / kPromo, w = blockIdx.x % kPromo, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float4* src = reinterpret_cast<const float4*>(a.part) +
+                      (static_cast<int64_t>(tile) * a.parts * kPromo + w) * 16 * 32 + warp * 4 * 32 + lane;
+  float4 v[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = src[c * 32];
+#pragma unroll 4
+  for (int p = 1; p < a.parts; ++p) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 x = src[static_cast<int64_t>(p) * kPromo * 16 * 32 + c * 32];
+      v[c].x += x.x; v[c].y += x.y; v[c].z += x.z; v[c].w += x.w;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) *reinterpret_cast<float4*>(&rows[lane][(warp * 4 + c) * 4]) = v[c];
+  __syncthreads();
+  int mt, nt;
+  tile_coords(a, a.full + tile, mt, nt);
+  const int r = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 16;
+  const int m = mt * kBM + (w & 3) * 32 + r, n = nt * 256 + (w >> 2) * 64 + c0;
+  if (m >= a.M || n >= a.N) return;
+  const int64_t o = static_cast<int64_t>(m) * a.ldo + n;
+  float y[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) y[e] = rows[r][c0 + e] + (a.bias != nullptr && n + e < a.N ? __ldg(a.bias + n + e) : 0.f);
+  if (a.vec_out && n + 16 <= a.N) {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + o * ES);
+#pragma unroll
+    for (int q = 0; q < ES; ++q) {
+      uint4 u;
+#pragma unroll
+      for (int e = 0; e < 16 / ES; e += 2)
+        stage2<ODT>(reinterpret_cast<uint8_t*>(&u) + e * ES, y[q * (16 / ES) + e], y[q * (16 / ES) + e + 1]);
+      dst[q] = u;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (n + e < a.N) store1<ODT>(a.out, o + e, y[e]);
   }
 }
 
@@ -588,11 +707,48 @@ bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t K, int64_t
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
+// Which kernel runs a product, and how its tiles are shared out.
+struct Plan {
+  enum { kFew16, kFew32, kWide, kNarrow, kShared } kind;
+  int ranks = 1, full = 0, parts = 1;
+  size_t workspace = 0;   // partial sums
+};
+
+Plan plan_product(int64_t M, int64_t N, int64_t kb) {
+  Plan p{};
+  // Few rows: the kernel that streams the weight (N = 7168, K = 5376: M = 32 in
+  // 12.7 us against 16.7 with 128-row tiles; at M = 64 it would take 21 us).
+  if (M <= 32) {
+    p.kind = M <= 16 ? Plan::kFew16 : Plan::kFew32;
+    return p;
+  }
+  // Time on the busiest SM in k-blocks of a 128 x 256 tile.  A 128 x 128 tile
+  // takes 0.55 of that (it reads twice the A bytes per MMA).  The last, partial
+  // round of 256-column tiles is split along K over all SMs where that takes
+  // more than 40 k-blocks off it: about 22 go to partial sums and their join,
+  // and few tiles alone run faster than a full round (1000 x 5376 x 14336: 168
+  // tiles, 148 whole and 20 in seven parts, 103 -> 84 us; 4096 x 7168 x 5376,
+  // 39 k-blocks, 156 -> 166 us if it were split).
+  const int64_t sms = sm_count(), mt = (M + 127) / 128;
+  const int64_t t256 = mt * ((N + 255) / 256), t128 = mt * ((N + 127) / 128);
+  const int64_t rest = t256 % sms, parts = rest ? min(sms / rest, kb / 2) : 1;
+  int64_t wide = (t256 + sms - 1) / sms * kb;
+  const int64_t saved = kb - (parts > 0 ? (kb + parts - 1) / parts : kb);
+  if (t256 > sms && saved > 40) {
+    wide -= saved - 22;
+    p.full = static_cast<int>(t256 - rest);
+    p.parts = static_cast<int>(parts);
+    p.workspace = static_cast<size_t>(rest) * parts * 128 * 256 * sizeof(float);
+  }
+  if (20 * wide <= 11 * ((t128 + sms - 1) / sms) * kb) {
+    p.kind = Plan::kWide;
+    return p;
+  }
+  p = Plan{};
+  // Tiles for less than half of the SMs: clusters share their k-blocks.
+  p.ranks = static_cast<int>(min(min(sms / t128, int64_t{8}), kb / 4));
+  p.kind = p.ranks >= 2 ? Plan::kShared : Plan::kNarrow;
+  return p;
 }
 
 struct Operands {
@@ -618,8 +774,8 @@ cudaError_t launch_cluster(K kernel, unsigned ctas, int threads, int smem, int r
   return cudaLaunchKernelEx(&cfg, kernel, m0, m1, a);
 }
 
-template <int BN, int ODT, bool SPLIT>
-cudaError_t launch(const Operands& op, MatmulArgs a, int ranks, cudaStream_t st) {
+template <int BN, int ODT, Share SHARE>
+cudaError_t launch(const Operands& op, MatmulArgs a, const Plan& plan, cudaStream_t st) {
   CUtensorMap ma, mb;
   if (!make_map(&ma, op.a, a.M, op.K, op.lda, kBM) || !make_map(&mb, op.b, a.N, op.K, op.ldb, BN))
     return cudaErrorInvalidValue;
@@ -627,16 +783,22 @@ cudaError_t launch(const Operands& op, MatmulArgs a, int ranks, cudaStream_t st)
   a.nt = (a.N + BN - 1) / BN;
   a.tiles = a.mt * a.nt;
   a.group = 16;
-  a.ranks = ranks;
-  auto k = matmul_blocks_kernel<BN, ODT, SPLIT>;
+  a.ranks = plan.ranks;
+  a.full = plan.full;
+  a.parts = plan.parts;
+  auto k = matmul_blocks_kernel<BN, ODT, SHARE>;
   const int smem = static_cast<int>(sizeof(MmSmem<BN>)) + 1024;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  if constexpr (!SPLIT) {
-    k<<<static_cast<unsigned>(min(a.tiles, sm_count())), MmCfg<BN>::kThreads, smem, st>>>(ma, mb, a);
-    return cudaGetLastError();
+  if constexpr (SHARE == kCluster)
+    return launch_cluster(k, static_cast<unsigned>(a.tiles) * plan.ranks, MmCfg<BN>::kThreads, smem, plan.ranks, st, ma, mb, a);
+  k<<<static_cast<unsigned>(min(a.tiles, sm_count())), MmCfg<BN>::kThreads, smem, st>>>(ma, mb, a);
+  e = cudaGetLastError();
+  if constexpr (SHARE == kParts) {
+    if (e == cudaSuccess)
+      e = launch_after(matmul_blocks_join_kernel<ODT>, dim3((a.tiles - a.full) * MmCfg<256>::kPromo), 128, 0, st, true, a);
   }
-  return launch_cluster(k, static_cast<unsigned>(a.tiles) * ranks, MmCfg<BN>::kThreads, smem, ranks, st, ma, mb, a);
+  return e;
 }
 
 template <int MN, int ODT>
@@ -657,20 +819,15 @@ cudaError_t launch_few(const Operands& op, const MatmulArgs& m, cudaStream_t st)
 }
 
 template <int ODT>
-cudaError_t dispatch(const Operands& op, const MatmulArgs& a, cudaStream_t st) {
-  // Few rows: the kernel that streams the weight (N = 7168, K = 5376: M = 32 in
-  // 12.7 us against 16.7 with 128-row tiles; at M = 64 it would take 21 us).
-  if (a.M <= 16) return launch_few<16, ODT>(op, a, st);
-  if (a.M <= 32) return launch_few<32, ODT>(op, a, st);
-  // A 256-column tile reads half the A bytes per MMA, a 128-column tile of the
-  // same k-block takes 0.55 of its time: the one with the shorter run of whole
-  // tiles on the busiest SM.
-  const int64_t sms = sm_count(), mt = (a.M + 127) / 128;
-  const int64_t t256 = mt * ((a.N + 255) / 256), t128 = mt * ((a.N + 127) / 128);
-  if (20 * ((t256 + sms - 1) / sms) <= 11 * ((t128 + sms - 1) / sms)) return launch<256, ODT, false>(op, a, 1, st);
-  // Tiles for less than half of the SMs: clusters share their k-blocks.
-  const int ranks = static_cast<int>(min(min(sms / t128, int64_t{8}), static_cast<int64_t>(a.kb / 4)));
-  return ranks >= 2 ? launch<128, ODT, true>(op, a, ranks, st) : launch<128, ODT, false>(op, a, 1, st);
+cudaError_t dispatch(const Operands& op, const MatmulArgs& a, const Plan& plan, cudaStream_t st) {
+  switch (plan.kind) {
+    case Plan::kFew16: return launch_few<16, ODT>(op, a, st);
+    case Plan::kFew32: return launch_few<32, ODT>(op, a, st);
+    case Plan::kWide:
+      return plan.parts > 1 ? launch<256, ODT, kParts>(op, a, plan, st) : launch<256, ODT, kWhole>(op, a, plan, st);
+    case Plan::kNarrow: return launch<128, ODT, kWhole>(op, a, plan, st);
+    default: return launch<128, ODT, kCluster>(op, a, plan, st);
+  }
 }
 
 int arg_error(const char* msg) {
@@ -695,11 +852,16 @@ cudaError_t matmul_blocks_status(int* code, int* where, int* block, bool reset) 
 
 }  // namespace vcattn
 
+extern "C" VCATTN_API size_t vcattn_matmul_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > (int64_t{1} << 30) || N > (int64_t{1} << 30) || K > (int64_t{1} << 30)) return 0;
+  return vcattn::plan_product(M, N, (K + vcattn::kBK - 1) / vcattn::kBK).workspace;
+}
+
 extern "C" VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float* a_scale, int64_t as_m,
                                                int64_t as_k, const uint8_t* b8, int64_t ldb, const float* b_scale,
                                                int64_t bs_n, int64_t bs_k, int64_t M, int64_t N, int64_t K,
                                                const float* bias, void* out, int out_dtype, int64_t ldo,
-                                               void* stream) {
+                                               void* workspace, size_t workspace_bytes, void* stream) {
   using namespace vcattn;
   clear_error();
   if (fault_injected("vcattn_matmul_blocks"))
@@ -722,11 +884,16 @@ extern "C" VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, c
   a.bias = bias; a.out = out; a.ldo = ldo; a.M = static_cast<int>(M); a.N = static_cast<int>(N);
   a.kb = static_cast<int>((K + kBK - 1) / kBK);
   a.vec_out = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (ldo * es) % 16 == 0;
+  const Plan plan = plan_product(M, N, a.kb);
+  if (plan.workspace > 0 &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < plan.workspace))
+    return record_error(VCATTN_ERR_WORKSPACE, "vcattn_matmul_blocks: workspace too small");
+  a.part = static_cast<float*>(workspace);
   const Operands op{a8, b8, lda, ldb, K};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = out_dtype == VCATTN_DTYPE_BF16  ? dispatch<VCATTN_DTYPE_BF16>(op, a, st)
-                        : out_dtype == VCATTN_DTYPE_F16 ? dispatch<VCATTN_DTYPE_F16>(op, a, st)
-                                                        : dispatch<VCATTN_DTYPE_F32>(op, a, st);
+  const cudaError_t e = out_dtype == VCATTN_DTYPE_BF16  ? dispatch<VCATTN_DTYPE_BF16>(op, a, plan, st)
+                        : out_dtype == VCATTN_DTYPE_F16 ? dispatch<VCATTN_DTYPE_F16>(op, a, plan, st)
+                                                        : dispatch<VCATTN_DTYPE_F32>(op, a, plan, st);
   if (e != cudaSuccess)
     return record_error(VCATTN_ERR_CUDA, (std::string("vcattn_matmul_blocks: ") + cudaGetErrorString(e)).c_str());
   return VCATTN_OK;

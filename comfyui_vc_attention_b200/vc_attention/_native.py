@@ -131,7 +131,8 @@ _SIGNATURES = {
                                        c_void_p, c_int64, c_int64, c_void_p]),
     "vcattn_matmul_blocks": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                      c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,
-                                     c_int64, c_void_p]),
+                                     c_int64, c_void_p, c_size_t, c_void_p]),
+    "vcattn_matmul_blocks_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "vcattn_attn_packed_workspace_bytes": (c_size_t, [POINTER(PackedWork), c_int, c_int, c_int]),
     "vcattn_attn_packed": (c_int, [POINTER(BHND), POINTER(BHND), POINTER(BHND), c_int, c_int, c_int, c_int, c_int,
                                    c_int, POINTER(PackedWork), c_int, c_float, POINTER(BHND), c_void_p, c_size_t,

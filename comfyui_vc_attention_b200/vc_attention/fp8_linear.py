@@ -131,10 +131,15 @@ def matmul_blocks(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = Non
             raise ValueError(f"out must be ({m}, {n}) {dtype} on {dev} with contiguous columns")
         ldo = out.stride(0) if m > 1 else max(n, 1)
     (sam, sak), (sbn, sbk) = a.scale.stride(), b.scale.stride()
+    lib, wp = N.lib(), None
     with on_device(dev):
-        N.check("vcattn_matmul_blocks", N.lib().vcattn_matmul_blocks(
+        need = lib.vcattn_matmul_blocks_workspace_bytes(m, n, k) if m > 32 else 0   # (few rows never need one)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            wp = ws.data_ptr()
+        N.check("vcattn_matmul_blocks", lib.vcattn_matmul_blocks(
             ac.data_ptr(), lda, a.scale.data_ptr(), sam, sak, bc.data_ptr(), ldb, b.scale.data_ptr(), sbn, sbk, m, n, k,
-            bp, out.data_ptr(), odt, ldo, stream(dev)))
+            bp, out.data_ptr(), odt, ldo, wp, need, stream(dev)))
     return out
 
 

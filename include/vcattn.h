@@ -362,12 +362,14 @@ VCATTN_API int vcattn_quantize_blocks(const void* x, int dtype, int64_t M, int64
  * a (M, K) and b (N, K) E4M3 codes with row pitches lda, ldb (multiples of 16,
  * 16-byte aligned); a_scale (M, ceil(K/128)) and b_scale (ceil(N/128),
  * ceil(K/128)) fp32 with element strides; bias (N,) fp32 or NULL.  fp32 sums,
- * one rounding to out_dtype.  Bounded waits report through
+ * one rounding to out_dtype.  The workspace (16-byte aligned) holds the partial
+ * sums of split tiles; its size may be 0.  Bounded waits report through
  * vcattn_attn_status as 400 + site. */
+VCATTN_API size_t vcattn_matmul_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K);
 VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float* a_scale, int64_t as_m, int64_t as_k,
                          const uint8_t* b8, int64_t ldb, const float* b_scale, int64_t bs_n, int64_t bs_k,
                          int64_t M, int64_t N, int64_t K, const float* bias, void* out, int out_dtype,
-                         int64_t ldo, void* stream);
+                         int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- exact attention over packed sequences ----------------------------------
  * Sequences of different lengths lie one after the other in q / out

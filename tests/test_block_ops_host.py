@@ -152,13 +152,16 @@ def test_c_entry_points_check_their_arguments():
         assert quant(**kw) == N.ERR_ARG and text in lib.vcattn_last_error(), kw
     assert quant(m=0, x=None) == N.OK
 
-    def mm(a=P, lda=128, m=4, n=8, k=128, dt=0, ldo=8, out=P):
-        return lib.vcattn_matmul_blocks(a, lda, P, 1, 4, P, 128, P, 1, 1, m, n, k, None, out, dt, ldo, None)
+    def mm(a=P, lda=128, m=4, n=8, k=128, dt=0, ldo=8, out=P, ldb=128):
+        return lib.vcattn_matmul_blocks(a, lda, P, 1, 4, P, ldb, P, 1, 1, m, n, k, None, out, dt, ldo, None, 0, None)
 
     for kw, text in ((dict(a=None), b"null"), (dict(a=P + 1), b"aligned"), (dict(lda=100), b"aligned"), (dict(k=0), b"range"),
                      (dict(dt=7), b"dtype"), (dict(ldo=4), b"stride"), (dict(out=P + 1), b"misaligned")):
         assert mm(**kw) == N.ERR_ARG and text in lib.vcattn_last_error(), kw
     assert mm(m=0) == N.OK
+    assert lib.vcattn_matmul_blocks_workspace_bytes(1000, 5376, 14336) == 20 * 7 * 128 * 256 * 4   # on 148 SMs
+    assert mm(m=1000, n=5376, k=14336, lda=14336, ldb=14336, ldo=5376) == N.ERR_WORKSPACE
+    assert lib.vcattn_matmul_blocks_workspace_bytes(1, 14336, 5376) == 0
 
     def attn(q=None, dtype=0, hq=4, hk=2, D=64, tiles=P, slots=0, scale=0.1, ws=None, wsb=0, n=1):
         work = N.PackedWork((None, tiles, None), (None,) * 3, (0, n, 0), (0, 0, 0), (0, slots, 0))

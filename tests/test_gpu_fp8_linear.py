@@ -112,7 +112,7 @@ def _check(out, a, b, bias):
 @pytest.mark.parametrize("m,n,k", [
     (1, 128, 128), (1, 5376, 7168), (2, 8, 16), (7, 200, 304), (16, 1, 128), (17, 129, 256), (33, 384, 1040),
     (64, 1000, 512), (65, 640, 2048), (129, 257, 144), (128, 256, 128), (333, 1536, 640), (1000, 5376, 384),
-    (2100, 2304, 256), (1, 3, 5376)])
+    (2100, 2304, 256), (1, 3, 5376), (1000, 5376, 6272), (1021, 5302, 6400)])
 def test_product(dtype, m, n, k):
     from comfyui_vc_attention_b200.vc_attention import matmul_blocks
     a, b = _blocks(m, k, 1, 1), _blocks(n, k, 128, 2)
