@@ -62,7 +62,7 @@ def _run(ql, kl, hq, hk, d, dtype, causal, **kw):
 LENGTHS = [
     ([1], [1]), ([1], [64]), ([1], [65]), ([64], [64]), ([63], [129]), ([65], [63]), ([128], [128]), ([257], [257]),
     ([1, 77, 0, 200, 333], [1, 77, 0, 200, 333]), ([5, 0, 3], [0, 9, 2]), ([130, 1, 17], [1, 1000, 400]),
-    ([300], [20]), ([1, 1, 1, 1], [2500, 1, 129, 640]), ([129, 255, 256], [511, 255, 1024]), ([700], [1500])]
+    ([300], [20]), ([700, 64, 90, 513, 300], [20, 700, 64, 1100, 300]), ([1, 1, 1, 1], [2500, 1, 129, 640]), ([129, 255, 256], [511, 255, 1024]), ([700], [1500])]
 
 
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 64),
@@ -93,6 +93,12 @@ def test_long_sequence():
     _run([3000], [2990], 2, 2, 64, torch.float16, False)
 
 
+def test_many_items_per_sm():
+    """More (tile, head) pairs than SMs, of unlike lengths, so that every CTA works through several."""
+    _run([900, 64, 300, 1, 520, 0, 257], [1200, 64, 10, 300, 520, 5, 900], 56, 56, 64, torch.float16, True)
+    _run([1030, 256, 70], [1030, 2000, 1], 40, 8, 128, torch.bfloat16, False)
+
+
 def test_layouts_out_and_neighbours():
     """(H, T, D) and (T, H, D) buffers, views of a fused projection, a given output."""
     from comfyui_vc_attention_b200.vc_attention import packed_attention, packed_plan
@@ -119,9 +125,9 @@ def test_layouts_out_and_neighbours():
 def test_non_finite_neighbours_and_keys(d, causal):
     """Sequences do not see each other's infinities and NaN, whichever tile they share."""
     from comfyui_vc_attention_b200.vc_attention import packed_attention, packed_plan
-    ql, kl = [40, 150, 30, 300], [40, 200, 30, 300]
-    q, k, v = _inputs(ql, kl, 2, 1, d, torch.bfloat16)
-    plan = packed_plan(ql, kl, heads=2, kv_heads=1, head_dim=d, causal=causal)
+    ql, kl, hq, hk = [40, 150, 30, 300], [40, 200, 30, 300], 2, 1
+    q, k, v = _inputs(ql, kl, hq, hk, d, torch.bfloat16)
+    plan = packed_plan(ql, kl, heads=hq, kv_heads=hk, head_dim=d, causal=causal)
     want = packed_attention(q, k, v, plan)
     for value in (float("nan"), float("inf")):
         k2, v2, q2 = k.clone(), v.clone(), q.clone()
@@ -133,12 +139,12 @@ def test_non_finite_neighbours_and_keys(d, causal):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("lq,lk", [(1, 400), (100, 100), (300, 300), (200, 500)])
-def test_non_finite_keys_behind_the_causal_mask(lq, lk, d):
+@pytest.mark.parametrize("lq,lk,heads", [(1, 400, 2), (100, 100, 2), (300, 300, 2), (200, 500, 2), (400, 400, 200)])
+def test_non_finite_keys_behind_the_causal_mask(lq, lk, heads, d):
     """Rows before a key that is infinite or NaN (in k, v or both) do not see it."""
     from comfyui_vc_attention_b200.vc_attention import packed_attention, packed_plan
-    q, k, v = _inputs([lq], [lk], 2, 1, d, torch.bfloat16)
-    plan = packed_plan([lq], [lk], heads=2, kv_heads=1, head_dim=d, causal=True)
+    q, k, v = _inputs([lq], [lk], heads, heads // 2, d, torch.bfloat16)
+    plan = packed_plan([lq], [lk], heads=heads, kv_heads=heads // 2, head_dim=d, causal=True)
     want = packed_attention(q, k, v, plan)
     key = lk - max(1, lq // 3)           # the rows from lq - max(1, lq // 3) on see it
     first = lq - max(1, lq // 3)
@@ -189,6 +195,27 @@ def test_offsets_past_32_bits():
     assert views[0].stride(2) * (n - 1) > 2 ** 31
     plan = packed_plan([n], heads=h, head_dim=d, causal=True)
     _check(packed_attention(*views, plan), *views, [n], [n], True)
+
+
+def test_no_wait_ran_out():
+    """The tcgen05 kernels' status words after the calls above (and a few more)."""
+    import ctypes
+    from comfyui_vc_attention_b200.vc_attention import _native as N
+    _run([700, 3], [1500, 40], 4, 2, 128, torch.bfloat16, True)
+    c = [ctypes.c_int(-1) for _ in range(3)]
+    N.check("vcattn_attn_status", N.lib().vcattn_attn_status(*(ctypes.byref(x) for x in c), 0))
+    assert c[0].value == 0, [x.value for x in c]
+
+
+def test_broadcast_keys_and_overlapping_output():
+    """Keys expanded over the heads (stride 0) are copied; an expanded output is refused."""
+    from comfyui_vc_attention_b200.vc_attention import packed_attention, packed_plan
+    q, k, v = _inputs([70], [90], 4, 1, 64, torch.float16)
+    plan = packed_plan([70], [90], heads=4, kv_heads=4, head_dim=64)
+    ke, ve = k.expand(1, 4, 90, 64), v.expand(1, 4, 90, 64)
+    _check(packed_attention(q, ke, ve, plan), q, ke, ve, [70], [90], False)
+    with pytest.raises(ValueError):
+        packed_attention(q, ke, ve, plan, out=q[:, :1].expand(1, 4, 70, 64))
 
 
 def test_refusals():
