@@ -61,13 +61,14 @@ def quantize_blocks(x: torch.Tensor, rows: int = 1) -> Fp8Blocks:
         ldx = k
     dev = x.device
     ldc = -(-k // 16) * 16
-    codes = torch.empty((m, ldc), dtype=torch.float8_e4m3fn, device=dev)
+    # (empty_strided: half the host time of empty, and the padded pitch in one call)
+    codes = torch.empty_strided((m, k), (ldc, 1), dtype=torch.float8_e4m3fn, device=dev)
     mb = m if rows == 1 else -(-m // rows)
     scale = torch.empty_strided((mb, -(-k // BLOCK)), (1, mb), dtype=torch.float32, device=dev)
     with on_device(dev):
         N.check("vcattn_quantize_blocks", N.lib().vcattn_quantize_blocks(
             x2.data_ptr(), dt, m, k, max(ldx, k), rows, codes.data_ptr(), ldc, scale.data_ptr(), 1, mb, stream(dev)))
-    return Fp8Blocks(codes if ldc == k else codes[:, :k], scale, rows)
+    return Fp8Blocks(codes, scale, rows)
 
 
 def _code_rows(b: Fp8Blocks, name: str, rows: int):
@@ -123,8 +124,8 @@ def matmul_blocks(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = Non
     if odt is None:
         raise TypeError(f"unsupported dtype {dtype}")
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=dev)
         ldo = max(n, 1)
+        out = torch.empty_strided((m, n), (ldo, 1), dtype=dtype, device=dev)
     else:
         if out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or \
                 (m > 1 and out.stride(0) < n):
@@ -135,7 +136,7 @@ def matmul_blocks(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = Non
     with on_device(dev):
         need = lib.vcattn_matmul_blocks_workspace_bytes(m, n, k) if m > 32 else 0   # (few rows never need one)
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
             wp = ws.data_ptr()
         N.check("vcattn_matmul_blocks", lib.vcattn_matmul_blocks(
             ac.data_ptr(), lda, a.scale.data_ptr(), sam, sak, bc.data_ptr(), ldb, b.scale.data_ptr(), sbn, sbk, m, n, k,

@@ -212,7 +212,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     (qv, q), (kv, k), (vv, v) = view(q), view(k), view(v)   # (what a view points into lives until the launch)
     need, ws = plan.workspace_bytes, None
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
     with on_device(dev):
         N.check("vcattn_attn_packed", N.lib().vcattn_attn_packed(
             qv, kv, vv, DTYPES[dtype], plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d, plan.work, plan.causal,

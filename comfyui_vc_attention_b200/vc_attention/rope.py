@@ -106,15 +106,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
         refuse_grad("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     if not (q.is_cuda and k.is_cuda):
         raise RuntimeError("qk_norm_rope needs CUDA tensors (this build has no CPU path)")
-    qs, ks, dev = q.shape, k.shape, q.device
-    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[2:] != ks[2:]:
+    qs, ks, dev, dtype = q.shape, k.shape, q.device, q.dtype
+    if len(qs) != 4 or len(ks) != 4:
         raise ValueError(f"q and k must be (B, Hq, N, D) and (B, Hk, N, D), got {tuple(qs)}, {tuple(ks)}")
-    if q.dtype != k.dtype or k.device != dev:
-        raise ValueError("q and k must share a dtype and a device")
-    dt = DTYPES.get(q.dtype)
-    if dt is None:
-        raise TypeError(f"unsupported dtype {q.dtype}")
     b, hq, n, d = qs
+    if ks != (b, ks[1], n, d):
+        raise ValueError(f"q and k must be (B, Hq, N, D) and (B, Hk, N, D), got {tuple(qs)}, {tuple(ks)}")
+    if k.dtype != dtype or k.device != dev:
+        raise ValueError("q and k must share a dtype and a device")
+    dt = DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"unsupported dtype {dtype}")
     if d & 7 or not 8 <= d <= 256:
         raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {d}")
     if layout == "half":
