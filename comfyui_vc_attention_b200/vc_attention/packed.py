@@ -44,7 +44,12 @@ class _Shape(NamedTuple):
 FEW = _Shape(16, 64, 2 * SMS, 0, 0, 0)
 MID = _Shape(64, 64, 3 * SMS, 128, 100, 160)
 WIDE = _Shape(256, 128, SMS, 320, 450, 640)
-WIDE_FROM = 64   # queries of a sequence that goes to the tcgen05 kernel
+# A tcgen05 tile takes about 0.55 of a 64-row register-MMA tile over the same
+# keys, but covers one query head where that covers a group's.  8 sequences of
+# 4096 keys, 32 / 8 heads, in us, tcgen05 / register MMAs: 24 queries 107 / 98,
+# 32 107 / 100, 48 112 / 145, 128 114 / 367; 56 / 56 heads, 1024 keys: 16
+# queries (16-row tiles) 37 / 30, 24 38 / 58.
+WIDE_TILE = 0.55
 
 
 @dataclass(frozen=True)
@@ -167,8 +172,9 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
         raise ValueError("a sequence has 2^31 rows or more")
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     q0, k0 = np.cumsum(ql) - ql, np.cumsum(kl) - kl
-    wide, few = ql >= WIDE_FROM, ql * g <= FEW.rows
-    lists = ((few & ~wide, g, kv_heads, FEW), (~few & ~wide, g, kv_heads, MID), (wide, 1, heads, WIDE))
+    few = ql * g <= FEW.rows
+    wide = ~few & (WIDE_TILE * g < -(-ql * g // MID.rows))
+    lists = ((few, g, kv_heads, FEW), (~few & ~wide, g, kv_heads, MID), (wide, 1, heads, WIDE))
     made = [_tiles(q0[pick], ql[pick], k0[pick], kl[pick], group, hs, causal, shape)
             for pick, group, hs, shape in lists]
     need = sum(m[2] * hs * shape.rows * (head_dim + 2) * 4 for m, (_, _, hs, shape) in zip(made, lists))

@@ -62,7 +62,7 @@ def _run(ql, kl, hq, hk, d, dtype, causal, **kw):
 LENGTHS = [
     ([1], [1]), ([1], [64]), ([1], [65]), ([64], [64]), ([63], [129]), ([65], [63]), ([128], [128]), ([257], [257]),
     ([1, 77, 0, 200, 333], [1, 77, 0, 200, 333]), ([5, 0, 3], [0, 9, 2]), ([130, 1, 17], [1, 1000, 400]),
-    ([300], [20]), ([700, 64, 90, 513, 300], [20, 700, 64, 1100, 300]), ([1, 1, 1, 1], [2500, 1, 129, 640]), ([129, 255, 256], [511, 255, 1024]), ([700], [1500])]
+    ([300], [20]), ([300, 2, 30], [0, 0, 0]), ([700, 64, 90, 513, 300], [20, 700, 64, 1100, 300]), ([1, 1, 1, 1], [2500, 1, 129, 640]), ([129, 255, 256], [511, 255, 1024]), ([700], [1500])]
 
 
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 64),
