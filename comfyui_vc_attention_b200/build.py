@@ -5,7 +5,9 @@
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` (in parallel) and
 the objects link into ``comfyui_vc_attention_b200/libvcattn.so``.  The library
 exports only the C ABI of ``include/vcattn.h``; it does not link against torch.
-A source is recompiled when it, or any header, is newer than its object.
+The host side of the block operators (``csrc/host_ops.cpp``) is a Python
+extension over torch's tensors, ``vc_attention/_host_ops.so``, that calls that
+ABI.  A source is recompiled when it, or any header, is newer than its object.
 """
 
 from __future__ import annotations
@@ -24,6 +26,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 BUILD = os.path.join(REPO, "_build")
 LIB = os.path.join(PKG, "libvcattn.so")
+HOST_OPS = os.path.join(PKG, "vc_attention", "_host_ops.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
@@ -51,6 +54,27 @@ def _compile(src: str, obj: str, extra) -> str:
     return r.stderr
 
 
+def _host_ops(force: bool) -> None:
+    src = os.path.join(CSRC, "host_ops.cpp")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "vcattn.h")))
+    if not force and os.path.exists(HOST_OPS) and os.path.getmtime(HOST_OPS) >= newest:
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_host_ops",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in inc], src,
+           "-o", HOST_OPS + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for host_ops.cpp:\n{r.stderr}\n{r.stdout}")
+    os.replace(HOST_OPS + ".tmp", HOST_OPS)
+
+
 def build(force: bool = False, jobs: int = 0, verbose: bool = False, extra=()) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -62,14 +86,16 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False, extra=()) -
         objs.append(o)
         if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(s), hdr):
             todo.append((s, o))
-    if todo:
-        jobs = jobs or min(len(todo), os.cpu_count() or 4)
-        with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+    jobs = jobs or min(len(todo) + 1, os.cpu_count() or 4)
+    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        host = ex.submit(_host_ops, force)
+        if todo:
             futs = {ex.submit(_compile, s, o, list(extra)): s for s, o in todo}
             for f in cf.as_completed(futs):
                 msg = f.result()
                 if verbose and msg.strip():
                     print(f"[{os.path.basename(futs[f])}]\n{msg}", file=sys.stderr)
+        host.result()
     if todo or not os.path.exists(LIB):
         cmd = [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", LIB + ".tmp"]
         r = subprocess.run(cmd, capture_output=True, text=True)

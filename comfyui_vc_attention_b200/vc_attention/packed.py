@@ -13,6 +13,7 @@ register MMAs over the rows of a KV head's group for few).  Forward only.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Sequence, Tuple
@@ -21,7 +22,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from ._launch import DTYPES, on_device, out_view, refuse_grad, stream, view
+from ._host import host_ops
 
 __all__ = ["PackedPlan", "packed_plan", "packed_attention"]
 
@@ -65,6 +66,7 @@ class PackedPlan:
     joins: Tuple[torch.Tensor, ...]   # and of vcattn_packed_join records
     work: N.PackedWork                # the lists for the C ABI
     workspace_bytes: int              # partial results of one call
+    call: object                      # the same for the host extension
 
     @property
     def device(self) -> torch.device:
@@ -183,8 +185,11 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
     recs = torch.from_numpy(host).to(dev).split([len(m[i]) for i in (0, 1) for m in made])
     work = N.PackedWork(tuple(r.data_ptr() for r in recs[:3]), tuple(r.data_ptr() for r in recs[3:]),
                         tuple(len(r) for r in recs[:3]), tuple(len(r) for r in recs[3:]), tuple(m[2] for m in made))
-    return PackedPlan(heads, kv_heads, head_dim, bool(causal), int(ql.sum()), int(kl.sum()), recs[:3], recs[3:],
-                      work, need)
+    tq, tk = int(ql.sum()), int(kl.sum())
+    index = recs[0].device.index
+    call = host_ops().PackedCall(heads, kv_heads, tq, tk, head_dim, bool(causal), ctypes.addressof(work), need,
+                                 -1 if index is None else index)
+    return PackedPlan(heads, kv_heads, head_dim, bool(causal), tq, tk, recs[:3], recs[3:], work, need, call)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,
@@ -197,30 +202,4 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     writes ``out``.  Scores, statistics and sums are fp32; P is rounded to q's
     type for the second product.
     """
-    if torch.is_grad_enabled():
-        refuse_grad("packed_attention", q, k, v)
-    if not (q.is_cuda and k.is_cuda and v.is_cuda):
-        raise RuntimeError("packed_attention needs CUDA tensors (this build has no CPU path)")
-    d = plan.head_dim
-    want_q, want_k = (1, plan.heads, plan.total_q, d), (1, plan.kv_heads, plan.total_k, d)
-    if q.shape != want_q or k.shape != want_k or v.shape != want_k:
-        raise ValueError(f"the plan needs q {want_q} and k, v {want_k}, got {tuple(q.shape)}, {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}")
-    dtype, dev = q.dtype, q.device
-    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
-        raise ValueError(f"q, k, v must share bfloat16 or float16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if not dev == k.device == v.device == plan.device:
-        raise ValueError("q, k, v and the plan must be on one device")
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    ov, out = out_view(out, q, "out")
-    (qv, q), (kv, k), (vv, v) = view(q), view(k), view(v)   # (what a view points into lives until the launch)
-    need, ws = plan.workspace_bytes, None
-    if need:
-        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
-    with on_device(dev):
-        N.check("vcattn_attn_packed", N.lib().vcattn_attn_packed(
-            qv, kv, vv, DTYPES[dtype], plan.heads, plan.kv_heads, plan.total_q, plan.total_k, d, plan.work, plan.causal,
-            scale, ov, None if ws is None else ws.data_ptr(), need, stream(dev)))
-    return out
+    return host_ops().packed_attention(q, k, v, plan.call, scale, out)

@@ -18,8 +18,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _native as N
-from ._launch import DTYPES, on_device, out_view, refuse_grad, stream, view
+from ._host import host_ops
 
 __all__ = ["rope_tables", "qk_norm_rope"]
 
@@ -74,17 +73,6 @@ def rope_tables(positions: torch.Tensor, rot_dim: Union[int, Sequence[int]], the
     return (ang.cos() * mult).float().contiguous(), (ang.sin() * mult).float().contiguous()
 
 
-def _vector(w: torch.Tensor, d: int, device: torch.device, what: str) -> torch.Tensor:
-    """A (D,) weight as the kernel reads it: fp32, contiguous, 16-byte aligned."""
-    if w.shape != (d,):
-        raise ValueError(f"{what} must be ({d},), got {tuple(w.shape)}")
-    if w.device != device:
-        raise ValueError(f"{what} must be on {device}, got {w.device}")
-    if w.dtype != torch.float32:
-        w = w.to(torch.float32)
-    return w if w.stride(0) == 1 and w.data_ptr() & 15 == 0 else w.clone(memory_format=torch.contiguous_format)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] = None,
                  sin: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
                  k_weight: Optional[torch.Tensor] = None, *, layout: str = "half", eps: float = 1e-5,
@@ -102,62 +90,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     out: a (q, k) pair of tensors to write (may be the inputs).  Arithmetic in
     fp32, rounded once.
     """
-    if torch.is_grad_enabled():
-        refuse_grad("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
-    if not (q.is_cuda and k.is_cuda):
-        raise RuntimeError("qk_norm_rope needs CUDA tensors (this build has no CPU path)")
-    qs, ks, dev, dtype = q.shape, k.shape, q.device, q.dtype
-    if len(qs) != 4 or len(ks) != 4:
-        raise ValueError(f"q and k must be (B, Hq, N, D) and (B, Hk, N, D), got {tuple(qs)}, {tuple(ks)}")
-    b, hq, n, d = qs
-    if ks != (b, ks[1], n, d):
-        raise ValueError(f"q and k must be (B, Hq, N, D) and (B, Hk, N, D), got {tuple(qs)}, {tuple(ks)}")
-    if k.dtype != dtype or k.device != dev:
-        raise ValueError("q and k must share a dtype and a device")
-    dt = DTYPES.get(dtype)
-    if dt is None:
-        raise TypeError(f"unsupported dtype {dtype}")
-    if d & 7 or not 8 <= d <= 256:
-        raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {d}")
-    if layout == "half":
-        flags = N.ROPE_NORM if norm else 0
-    elif layout == "interleaved":
-        flags = N.ROPE_INTERLEAVED | (N.ROPE_NORM if norm else 0)
-    else:
-        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-    rot = tsb = tsn = 0
-    cp = sp = None
-    if cos is not None and sin is not None:
-        cs = cos.shape
-        if cs != sin.shape or len(cs) not in (2, 3) or cs[-2] != n or (len(cs) == 3 and cs[0] not in (1, b)):
-            raise ValueError(f"cos and sin must be ({n}, r/2) or ({b}, {n}, r/2), got {tuple(cs)}, {tuple(sin.shape)}")
-        if cos.device != dev or sin.device != dev:
-            raise ValueError(f"cos and sin must be on {dev}")
-        rot = 2 * cs[-1]
-        if rot & 15 or rot > d:
-            raise ValueError(f"the rotated channels must be a multiple of 16 up to {d}, got {rot}")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32:
-            cos, sin = cos.to(torch.float32), sin.to(torch.float32)
-        st = cos.stride()
-        if st != sin.stride() or st[-1] != 1 or (st[0] | st[-2]) & 3 or (cos.data_ptr() | sin.data_ptr()) & 15:
-            cos, sin = (x.clone(memory_format=torch.contiguous_format) for x in (cos, sin))
-            st = cos.stride()
-        tsn = st[-2]
-        tsb = st[0] if len(st) == 3 and cs[0] > 1 else 0
-        cp, sp = cos.data_ptr(), sin.data_ptr()
-    elif cos is not None or sin is not None:
-        raise ValueError("cos and sin are given together")
-    qw = kw = None
-    if q_weight is not None:
-        q_weight = _vector(q_weight, d, dev, "q_weight")
-        qw = q_weight.data_ptr()
-    if k_weight is not None:
-        k_weight = _vector(k_weight, d, dev, "k_weight")
-        kw = k_weight.data_ptr()
     oq, ok = (None, None) if out is None else out
-    (ov, oq), (pv, ok) = out_view(oq, q, "out[0]"), out_view(ok, k, "out[1]")
-    (qv, q), (kv, k) = view(q), view(k)   # (what a view points into lives until the launch)
-    with on_device(dev):
-        N.check("vcattn_qk_norm_rope", N.lib().vcattn_qk_norm_rope(
-            qv, kv, dt, b, hq, ks[1], n, d, qw, kw, cp, sp, tsb, tsn, rot, flags, eps, ov, pv, stream(dev)))
-    return oq, ok
+    return host_ops().qk_norm_rope(q, k, cos, sin, q_weight, k_weight, layout, eps, norm, oq, ok)
