@@ -380,6 +380,17 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         for (int c = 0; c < 16; ++c) dst[c * 32] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         continue;
       }
+      if (a.bias != nullptr) {
+        // this warp's 64 values, two per lane (one coalesced load each), then
+        // from lane to lane: 64 loads per thread cost 10 us of a 45 us product
+        const float b0 = n0 + lane < a.N ? __ldg(a.bias + n0 + lane) : 0.f;
+        const float b1 = n0 + 32 + lane < a.N ? __ldg(a.bias + n0 + 32 + lane) : 0.f;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          acc[c] += __shfl_sync(0xffffffffu, b0, c);
+          acc[32 + c] += __shfl_sync(0xffffffffu, b1, c);
+        }
+      }
       // rows through shared memory, so that whole 32-byte sectors go out
       constexpr int PC = 128 / ES;   // columns per pass
 #pragma unroll
@@ -390,12 +401,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
           uint4 w;
 #pragma unroll
           for (int e = 0; e < 16 / ES; e += 2) {
-            float v0 = acc[p * PC + c + e], v1 = acc[p * PC + c + e + 1];
-            if (a.bias != nullptr) {
-              v0 += np + c + e < a.N ? __ldg(a.bias + np + c + e) : 0.f;
-              v1 += np + c + e + 1 < a.N ? __ldg(a.bias + np + c + e + 1) : 0.f;
-            }
-            stage2<ODT>(reinterpret_cast<uint8_t*>(&w) + e * ES, v0, v1);
+            stage2<ODT>(reinterpret_cast<uint8_t*>(&w) + e * ES, acc[p * PC + c + e], acc[p * PC + c + e + 1]);
           }
           *reinterpret_cast<uint4*>(stage + lane * Cfg::kOutPitch + c * ES) = w;
         }
