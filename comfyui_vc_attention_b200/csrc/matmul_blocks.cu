@@ -821,9 +821,12 @@ cudaError_t launch_few(const Operands& op, const MatmulArgs& m, cudaStream_t st)
   const int smem = static_cast<int>(sizeof(FewSmem<MN>)) + 1024;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  // CTAs per row tile: enough for the CTAs that fit on every SM, at least two k-blocks each
+  // CTAs per row tile: as many as start at once (three or two fit on an SM, but
+  // whole clusters do not fill every SM: N = 7168, K = 5376, 16 rows, 6 ranks
+  // 13.0 us, 7 ranks 17.7; 32 rows, 4 ranks 14.4, 6 ranks 19.2), at least two
+  // k-blocks each.
   const int tiles = (m.N + 127) / 128;
-  const int want = ((MN == 16 ? 3 : 2) * sm_count()) / tiles;
+  const int want = (MN == 16 ? 23 : 16) * sm_count() / 10 / tiles;
   const int ranks = max(1, min(min(8, want), m.kb / 2));
   return launch_cluster(k, static_cast<unsigned>(tiles) * ranks, 256, smem, ranks, st, mw, mx, a);
 }
