@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(128) matmul_blocks_join_kernel(const MatmulArg
 }
 
 // ---- few rows ------------------------------------------------------------------
-// For M up to 64 the weight's bytes bound the product.  Here the weight rows
+// For M up to 32 the weight's bytes bound the product.  Here the weight rows
 // are the MMA's 128 rows and the activations its MN columns, and the k-blocks
 // of a row tile are dealt to the CTAs of a cluster, so that every SM streams
 // weights; the partial sums meet in shared memory of the cluster and are added
@@ -726,8 +726,10 @@ struct Plan {
 
 Plan plan_product(int64_t M, int64_t N, int64_t kb) {
   Plan p{};
-  // Few rows: the kernel that streams the weight (N = 7168, K = 5376: M = 32 in
-  // 12.7 us against 16.7 with 128-row tiles; at M = 64 it would take 21 us).
+  // Few rows: the kernel that streams the weight.  K = 5376, N = 7168: 16 rows
+  // 13.0 us, 32 rows 14.4, 128-row tiles 16.4 (the form for 64 rows took 21).  Wide
+  // weights bring both sides together: N = 14336, 24 rows 20.6 against 27.8, 32 rows
+  // 22.4 against 20.5; N = 28672, 36.6 against 37.8 and 37.8 against 33.1.
   if (M <= 32) {
     p.kind = M <= 16 ? Plan::kFew16 : Plan::kFew32;
     return p;
