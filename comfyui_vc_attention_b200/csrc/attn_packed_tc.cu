@@ -412,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && !*abort) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
+        __syncwarp();   // the lanes part below, and the load of tensor memory is one of the whole warp
         float o[32];
         if (nh > 0) {
           tmem_ld32(to + 32 * c, o);
@@ -422,8 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (!live) continue;
-        if (bad) {
+        if (live && bad) {
           // the infinite and NaN values of the edge tiles, for the rows that see them
           const uint16_t* q = static_cast<const uint16_t*>(a.q) + head * a.qsh + static_cast<int64_t>(t.q0 + tok) * a.qsn;
           const int kvh = head / a.G;
@@ -441,11 +441,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (not_finite<DT>(v[e])) o[e] = fmaf(p, value16<DT>(v[e]), o[e]);
           }
         }
-        if (part) {
+        if (live && part) {
           float4* po = reinterpret_cast<float4*>(a.part_o + prow * D + 32 * c);
 #pragma unroll
           for (int e = 0; e < 8; ++e) po[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        } else {
+        } else if (live) {
           uint4* po = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + head * a.osh +
                                                static_cast<int64_t>(t.q0 + tok) * a.osn + 32 * c);
 #pragma unroll
