@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int seen = row_limit(t, a.causal, t.r0);   // keys below are seen by every row of the CTA
       for (int j = 0; j < n; ++j) {
         const int i = 2 * j + 1, s = i % kStages;
-        if (!mbar_wait(&sm.full[s], (i / kStages) & 1, abort, status, 7)) break;
+        if (!warp_wait(&sm.full[s], (i / kStages) & 1, abort, status, 7)) break;
         const int key0 = t.kb + j * kKeys;
         if (key0 + kKeys > min(seen, t.lk)) {
           bool wrote = false, found = false;
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l0 = 0.f, l1 = 0.f;
     bool ok = true;
     for (int j = 0; j < nh; ++j) {
-      if (!(ok = mbar_wait(&sm.s_full[h], j & 1, abort, status, 8))) break;
+      if (!(ok = warp_wait(&sm.s_full[h], j & 1, abort, status, 8))) break;
       tc_fence_after();
       float x[kKeys];
 #pragma unroll
@@ -402,14 +402,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (ok && nh > 0) ok = mbar_wait(&sm.o_full[h], 0, abort, status, 9);
+    if (ok && nh > 0) ok = warp_wait(&sm.o_full[h], 0, abort, status, 9);
     tc_fence_after();
     const float l = l0 + l1;
     const bool bad = *static_cast<volatile int*>(&sm.bad) != 0;
     const bool part = t.slot >= 0;
     const float inv = part ? 1.f : l != 0.f ? __fdiv_rn(1.f, l) : 0.f;   // (l is NaN where a score was)
     const int64_t prow = (static_cast<int64_t>(t.slot) * a.Hq + head) * (2 * kHalf) + h * kHalf + row;
-    if (ok && !*abort) {
+    if (__all_sync(0xffffffffu, ok && *abort == 0)) {
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         __syncwarp();   // the lanes part below, and the load of tensor memory is one of the whole warp

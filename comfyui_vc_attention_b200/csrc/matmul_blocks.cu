@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       load(pc.k0());
       for (int k = pc.k0(); k < pc.k1(a); k += kGroup, ++grp) {
         const int s = grp & 1;
-        if (grp >= 2 && !(ok = mbar_wait(&sm.s_empty[s], ((grp >> 1) + 1) & 1, abort, status, 5))) break;
+        if (grp >= 2 && !(ok = warp_wait(&sm.s_empty[s], ((grp >> 1) + 1) & 1, abort, status, 5))) break;
         *reinterpret_cast<float4*>(sm.scale[s][0][r]) = make_float4(x0[0] * y0[0], x0[1] * y0[1], x0[2] * y0[2], x0[3] * y0[3]);
         *reinterpret_cast<float4*>(sm.scale[s][0][r + 64]) = make_float4(x1[0] * y0[0], x1[1] * y0[1], x1[2] * y0[2], x1[3] * y0[3]);
         if constexpr (BN == 256) {
@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       float acc[64];
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-      for (int k = pc.k0(); ok && k < pc.k1(a); k += kGroup) {
-        if (!(ok = mbar_wait(&sm.s_full[g], g_par, abort, status, 4))) break;
+      for (int k = pc.k0(); k < pc.k1(a); k += kGroup) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.s_full[g], g_par, abort, status, 4));
+        if (!ok) break;
         const float4 s4 = *reinterpret_cast<const float4*>(scale + g * (BN / 128 * kBM * kGroup));
         warp_arrive(&sm.s_empty[g], lane);
         g ^= 1;
@@ -345,7 +346,9 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
         const float s[kGroup] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
-          if (k + u >= pc.k1(a) || !(ok = mbar_wait(&sm.t_full[b], b_par, abort, status, 6))) break;
+          if (k + u >= pc.k1(a)) break;
+          // (a lane that gave up keeps step with the others until the next vote; one here costs 2 %)
+          ok = ok && mbar_wait(&sm.t_full[b], b_par, abort, status, 6);
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -364,7 +367,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
           b_par ^= b == 0;
         }
       }
-      if (!ok || *abort) continue;
+      ok = __all_sync(0xffffffffu, ok && *abort == 0);
+      if (!ok) continue;
       if constexpr (SHARE == kCluster) {
         // this rank's sums over the operand stages (every MMA has read them)
         float* part = reinterpret_cast<float*>(sm.a) + (wq * 32 + lane) * Cfg::kPartPitch + quarter * 64;
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(256, MN == 16 ? 3 : 2)
       }
       asm volatile("bar.sync 1, 128;\n" ::: "memory");   // the scales of this block are written, those of it - 1 read
       // (a warp that gave up keeps step with the others' barrier)
-      ok = ok && mbar_wait(&sm.t_full[b], (it >> 1) & 1, abort, status, 14);
+      ok = ok && warp_wait(&sm.t_full[b], (it >> 1) & 1, abort, status, 14);
       tc_fence_after();
       float x[MN];
 #pragma unroll

@@ -19,6 +19,14 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+// mbar_wait by a whole warp with one answer for all lanes: where a wait runs
+// out, lanes that differ in when they saw it would take different branches
+// around the warp-wide instructions that follow.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, DevStatus* status,
+                                          int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, where));
+}
+
 // ---- packed fp32 helpers ---------------------------------------------------
 __device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
   asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
