@@ -128,6 +128,8 @@ const float* weight(const OptTensor& w, int64_t d, const at::Device& dev, const 
   return static_cast<const float*>(keep.data_ptr());
 }
 
+constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;
+
 std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& cos_in, const OptTensor& sin_in,
                                         const OptTensor& q_weight, const OptTensor& k_weight, const std::string& layout,
                                         double eps, bool norm, const OptTensor& out_q, const OptTensor& out_k) {
@@ -142,6 +144,10 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
   const int dt = dtype_code(q.scalar_type());
   const int64_t b = q.size(0), n = q.size(2), d = q.size(3);
   CHECK_VALUE(d % 8 == 0 && d >= 8 && d <= 256, "head_dim must be a multiple of 8 up to 256, got ", d);
+  // (the C entry point takes these as int: checked here, before they are narrowed)
+  const int64_t heads = q.size(1) + k.size(1);
+  CHECK_VALUE(b <= kMaxRows && n <= kMaxRows && heads <= kMaxRows && b * n <= kMaxRows / std::max<int64_t>(heads, 1),
+              "2^31 head rows or more: q ", q.sizes(), ", k ", k.sizes());
   CHECK_VALUE(layout == "half" || layout == "interleaved", "layout must be 'half' or 'interleaved', got '", layout, "'");
   const int flags = (layout == "half" ? 0 : VCATTN_ROPE_INTERLEAVED) | (norm ? VCATTN_ROPE_NORM : 0);
   CHECK_VALUE(cos_in.has_value() == sin_in.has_value(), "cos and sin are given together");

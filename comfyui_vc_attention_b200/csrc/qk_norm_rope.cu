@@ -280,7 +280,8 @@ extern "C" VCATTN_API int vcattn_qk_norm_rope(const vcattn_bhnd* q, const vcattn
   if (D < 8 || D > 256 || D % 8) return arg_error("D must be a multiple of 8 up to 256");
   if (rot < 0 || rot > D || rot % 16) return arg_error("rot must be a multiple of 16 up to D");
   if (flags & ~(VCATTN_ROPE_INTERLEAVED | VCATTN_ROPE_NORM)) return arg_error("unknown flag");
-  if (static_cast<int64_t>(B) * N == 0 || Hq + Hk == 0) return VCATTN_OK;
+  const int64_t heads = static_cast<int64_t>(Hq) + Hk;
+  if (static_cast<int64_t>(B) * N == 0 || heads == 0) return VCATTN_OK;
   const int es = dtype == VCATTN_DTYPE_F32 ? 4 : 2;
   if ((Hq > 0 && (!view_fits(q, es) || !view_fits(q_out, es))) || (Hk > 0 && (!view_fits(k, es) || !view_fits(k_out, es))))
     return arg_error("q, k and the outputs must be 16-byte aligned with strides of 16-byte multiples");
@@ -309,7 +310,7 @@ extern "C" VCATTN_API int vcattn_qk_norm_rope(const vcattn_bhnd* q, const vcattn
   const int t0 = Hq > 0 ? 0 : 1;
   a.token_major = a.xsh[t0] <= a.xsn[t0];
   // (a warp takes four heads or more, so this bounds its count of groups)
-  if (static_cast<int64_t>(B) * N >= (int64_t{1} << 31) / (Hq + Hk)) return arg_error("2^31 head rows or more");
+  if (static_cast<int64_t>(B) * N > ((int64_t{1} << 31) - 1) / heads) return arg_error("2^31 head rows or more");
   const bool half = !(flags & VCATTN_ROPE_INTERLEAVED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == VCATTN_DTYPE_BF16  ? launch_dtype<VCATTN_DTYPE_BF16>(a, half, st)
