@@ -248,7 +248,7 @@ extern "C" VCATTN_API int vcattn_quantize_blocks(const void* x, int dtype, int64
   if (dtype != VCATTN_DTYPE_BF16 && dtype != VCATTN_DTYPE_F16 && dtype != VCATTN_DTYPE_F32)
     return arg_error("unsupported dtype");
   if (block_rows != 1 && block_rows != kBlk) return arg_error("block_rows must be 1 or 128");
-  if (M < 0 || K < 0 || K > (int64_t{1} << 30)) return arg_error("size out of range");
+  if (M < 0 || K < 0 || M > (int64_t{1} << 36) || K > (int64_t{1} << 30)) return arg_error("size out of range");
   if (M == 0 || K == 0) return VCATTN_OK;
   if (!x || !codes || !scale) return arg_error("null pointer");
   if (ldx < K || ldc < K) return arg_error("row stride below the row length");
