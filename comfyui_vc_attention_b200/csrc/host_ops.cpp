@@ -10,6 +10,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/extension.h>
 
+#include <memory>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -21,24 +22,23 @@ namespace {
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 
-struct Entry {
+// What one loaded copy of the package brings: the library's entry points and
+// its `check`, which raises that copy's VCAttnError with the library's message.
+struct Library {
   decltype(&vcattn_qk_norm_rope) qk_norm_rope = nullptr;
   decltype(&vcattn_quantize_blocks) quantize_blocks = nullptr;
   decltype(&vcattn_matmul_blocks) matmul_blocks = nullptr;
   decltype(&vcattn_matmul_blocks_workspace_bytes) matmul_workspace = nullptr;
   decltype(&vcattn_attn_packed) attn_packed = nullptr;
-} entry;
+  py::object check;
 
-template <typename F> F address(const py::dict& d, const char* name) {
-  return reinterpret_cast<F>(d[name].cast<uintptr_t>());
-}
+  void status(int rc, const char* fn) const {
+    if (rc != VCATTN_OK) check(fn, rc);
+  }
+};
 
-void bind(const py::dict& d) {
-  entry.qk_norm_rope = address<decltype(entry.qk_norm_rope)>(d, "vcattn_qk_norm_rope");
-  entry.quantize_blocks = address<decltype(entry.quantize_blocks)>(d, "vcattn_quantize_blocks");
-  entry.matmul_blocks = address<decltype(entry.matmul_blocks)>(d, "vcattn_matmul_blocks");
-  entry.matmul_workspace = address<decltype(entry.matmul_workspace)>(d, "vcattn_matmul_blocks_workspace_bytes");
-  entry.attn_packed = address<decltype(entry.attn_packed)>(d, "vcattn_attn_packed");
+template <typename F> void address(const py::dict& d, const char* name, F& f) {
+  f = reinterpret_cast<F>(d[name].cast<uintptr_t>());
 }
 
 // ---- errors -------------------------------------------------------------------
@@ -51,11 +51,6 @@ template <typename... A> std::string text(const A&... a) {
   do {                         \
     if (!(cond)) throw py::value_error(text(__VA_ARGS__)); \
   } while (0)
-
-void check_status(int rc, const char* fn) {
-  if (rc != VCATTN_OK)   // raises VCAttnError with the library's message
-    py::module_::import("comfyui_vc_attention_b200.vc_attention._native").attr("check")(fn, rc);
-}
 
 void need_cuda(bool cuda, const char* fn) {
   if (!cuda) throw std::runtime_error(text(fn, " needs CUDA tensors (this build has no CPU path)"));
@@ -130,7 +125,7 @@ const float* weight(const OptTensor& w, int64_t d, const at::Device& dev, const 
 
 constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;
 
-std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& cos_in, const OptTensor& sin_in,
+std::tuple<Tensor, Tensor> qk_norm_rope(const Library& lib, const Tensor& q, const Tensor& k, const OptTensor& cos_in, const OptTensor& sin_in,
                                         const OptTensor& q_weight, const OptTensor& k_weight, const std::string& layout,
                                         double eps, bool norm, const OptTensor& out_q, const OptTensor& out_k) {
   refuse_grad("qk_norm_rope", q, k);
@@ -180,7 +175,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
   const Tensor oq = out_rows(out_q, q, "out[0]"), ok = out_rows(out_k, k, "out[1]");
   const View vq = view(q), vk = view(k);
   const vcattn_bhnd wq_out = bhnd(oq), wk_out = bhnd(ok);
-  check_status(entry.qk_norm_rope(&vq.v, &vk.v, dt, static_cast<int>(b), static_cast<int>(q.size(1)),
+  lib.status(lib.qk_norm_rope(&vq.v, &vk.v, dt, static_cast<int>(b), static_cast<int>(q.size(1)),
                                   static_cast<int>(k.size(1)), static_cast<int>(n), static_cast<int>(d), qw, kw,
                                   rot ? static_cast<const float*>(cos.data_ptr()) : nullptr,
                                   rot ? static_cast<const float*>(sin.data_ptr()) : nullptr, tsb, tsn,
@@ -193,7 +188,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
 constexpr int64_t kBlock = 128;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& x, int64_t rows) {
+std::tuple<Tensor, Tensor> quantize_blocks(const Library& lib, const Tensor& x, int64_t rows) {
   refuse_grad("quantize_blocks", x);
   need_cuda(x.is_cuda(), "quantize_blocks");
   CHECK_VALUE(rows == 1 || rows == kBlock, "rows must be 1 or ", kBlock, ", got ", rows);
@@ -208,7 +203,7 @@ std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& x, int64_t rows) {
   // (code rows 16 bytes apart at least, scales with rows side by side)
   const Tensor codes = at::empty_strided({m, k}, {ldc, 1}, x.options().dtype(at::kFloat8_e4m3fn));
   const Tensor scale = at::empty_strided({mb, ceil_div(k, kBlock)}, {1, mb}, x.options().dtype(at::kFloat));
-  check_status(entry.quantize_blocks(x2.data_ptr(), dt, m, k, ldx, static_cast<int>(rows),
+  lib.status(lib.quantize_blocks(x2.data_ptr(), dt, m, k, ldx, static_cast<int>(rows),
                                      static_cast<uint8_t*>(codes.data_ptr()), ldc, static_cast<float*>(scale.data_ptr()),
                                      1, mb, stream_of(x)),
                "vcattn_quantize_blocks");
@@ -235,7 +230,7 @@ Tensor code_rows(const Tensor& c, const Tensor& s, int64_t rows, int64_t want, c
   return t;
 }
 
-Tensor matmul_blocks(const Tensor& a, const Tensor& sa, int64_t a_rows, const Tensor& b, const Tensor& sb, int64_t b_rows,
+Tensor matmul_blocks(const Library& lib, const Tensor& a, const Tensor& sa, int64_t a_rows, const Tensor& b, const Tensor& sb, int64_t b_rows,
                      const OptTensor& bias_in, const py::object& dtype, const OptTensor& out_in) {
   refuse_grad("matmul_blocks", sa, sb);
   if (bias_in.has_value()) refuse_grad("matmul_blocks", *bias_in);
@@ -267,10 +262,10 @@ Tensor matmul_blocks(const Tensor& a, const Tensor& sa, int64_t a_rows, const Te
   } else {
     out = at::empty_strided({m, n}, {ldo, 1}, a.options().dtype(st));
   }
-  const size_t need = entry.matmul_workspace(m, n, k);
+  const size_t need = lib.matmul_workspace(m, n, k);
   Tensor ws;
   if (need > 0) ws = at::empty_strided({static_cast<int64_t>(need)}, {1}, a.options().dtype(at::kByte));
-  check_status(entry.matmul_blocks(static_cast<const uint8_t*>(ac.data_ptr()), lda, static_cast<const float*>(sa.data_ptr()),
+  lib.status(lib.matmul_blocks(static_cast<const uint8_t*>(ac.data_ptr()), lda, static_cast<const float*>(sa.data_ptr()),
                                    sa.stride(0), sa.stride(1), static_cast<const uint8_t*>(bc.data_ptr()), ldb,
                                    static_cast<const float*>(sb.data_ptr()), sb.stride(0), sb.stride(1), m, n, k,
                                    bias.defined() ? static_cast<const float*>(bias.data_ptr()) : nullptr, out.data_ptr(), odt,
@@ -290,7 +285,9 @@ struct PackedCall {
   int device;       // index, -1 for a plan on the CPU
 };
 
-Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const PackedCall& p, std::optional<double> scale,
+constexpr const char* kPackedCall = "vcattn packed call";
+
+Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, const Tensor& v, const PackedCall& p, std::optional<double> scale,
                         const OptTensor& out_in) {
   refuse_grad("packed_attention", q, k, v);
   need_cuda(q.is_cuda() && k.is_cuda() && v.is_cuda(), "packed_attention");
@@ -312,7 +309,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   const vcattn_bhnd vo = bhnd(out);
   Tensor ws;
   if (p.workspace > 0) ws = at::empty_strided({static_cast<int64_t>(p.workspace)}, {1}, q.options().dtype(at::kByte));
-  check_status(entry.attn_packed(&vq.v, &vk.v, &vv.v, dtype_code(st), p.heads, p.kv_heads, static_cast<int>(p.total_q),
+  lib.status(lib.attn_packed(&vq.v, &vk.v, &vv.v, dtype_code(st), p.heads, p.kv_heads, static_cast<int>(p.total_q),
                                  static_cast<int>(p.total_k), static_cast<int>(p.head_dim),
                                  reinterpret_cast<const vcattn_packed_work*>(p.work), p.causal ? 1 : 0,
                                  static_cast<float>(s), &vo, p.workspace ? ws.data_ptr() : nullptr, p.workspace,
@@ -321,17 +318,42 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   return out;
 }
 
+Tensor packed_attention_plan(const Library& lib, const Tensor& q, const Tensor& k, const Tensor& v, const py::object& call,
+                             std::optional<double> scale, const OptTensor& out) {
+  const void* p = PyCapsule_GetPointer(call.ptr(), kPackedCall);
+  if (p == nullptr) throw py::error_already_set();
+  return packed_attention(lib, q, k, v, *static_cast<const PackedCall*>(p), scale, out);
+}
+
+// f with its library.
+template <typename R, typename... A> auto with(std::shared_ptr<const Library> lib, R (*f)(const Library&, A...)) {
+  return [lib, f](A... a) -> R { return f(*lib, std::forward<A>(a)...); };
+}
+
+// The operators of `m`, on these entry points.  (Two copies of the package may
+// share this extension's code, so nothing of either is kept outside the module.)
+void bind(py::module_ m, const py::dict& d, py::object check) {
+  auto lib = std::make_shared<Library>();
+  address(d, "vcattn_qk_norm_rope", lib->qk_norm_rope);
+  address(d, "vcattn_quantize_blocks", lib->quantize_blocks);
+  address(d, "vcattn_matmul_blocks", lib->matmul_blocks);
+  address(d, "vcattn_matmul_blocks_workspace_bytes", lib->matmul_workspace);
+  address(d, "vcattn_attn_packed", lib->attn_packed);
+  lib->check = std::move(check);
+  m.def("qk_norm_rope", with(lib, &qk_norm_rope));
+  m.def("quantize_blocks", with(lib, &quantize_blocks));
+  m.def("matmul_blocks", with(lib, &matmul_blocks));
+  m.def("packed_attention", with(lib, &packed_attention_plan));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
-  m.def("qk_norm_rope", &qk_norm_rope);
-  m.def("quantize_blocks", &quantize_blocks);
-  m.def("matmul_blocks", &matmul_blocks);
-  m.def("packed_attention", &packed_attention);
-  py::class_<PackedCall>(m, "PackedCall")
-      .def(py::init([](int heads, int kv_heads, int64_t total_q, int64_t total_k, int64_t head_dim, bool causal,
-                       uintptr_t work, size_t workspace, int device) {
-        return PackedCall{heads, kv_heads, total_q, total_k, head_dim, causal, work, workspace, device};
-      }));
+  // (a capsule: a registered class could not be registered again by a second copy)
+  m.def("packed_call", [](int heads, int kv_heads, int64_t total_q, int64_t total_k, int64_t head_dim, bool causal,
+                          uintptr_t work, size_t workspace, int device) {
+    return py::capsule(new PackedCall{heads, kv_heads, total_q, total_k, head_dim, causal, work, workspace, device}, kPackedCall,
+                       [](PyObject* c) { delete static_cast<PackedCall*>(PyCapsule_GetPointer(c, kPackedCall)); });
+  });
 }

@@ -35,6 +35,6 @@ def host_ops():
             spec.loader.exec_module(mod)
         except ImportError as e:
             raise N.NativeUnavailable(f"failed to load {HOST_OPS_PATH}: {e}") from e
-        mod.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRY_POINTS})
+        mod.bind(mod, {name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _ENTRY_POINTS}, N.check)
         _mod = mod
     return _mod

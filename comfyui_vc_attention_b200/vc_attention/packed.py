@@ -187,7 +187,7 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
                         tuple(len(r) for r in recs[:3]), tuple(len(r) for r in recs[3:]), tuple(m[2] for m in made))
     tq, tk = int(ql.sum()), int(kl.sum())
     index = recs[0].device.index
-    call = host_ops().PackedCall(heads, kv_heads, tq, tk, head_dim, bool(causal), ctypes.addressof(work), need,
+    call = host_ops().packed_call(heads, kv_heads, tq, tk, head_dim, bool(causal), ctypes.addressof(work), need,
                                  -1 if index is None else index)
     return PackedPlan(heads, kv_heads, head_dim, bool(causal), tq, tk, recs[:3], recs[3:], work, need, call)
 
