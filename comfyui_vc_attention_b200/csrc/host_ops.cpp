@@ -5,15 +5,20 @@
 // 16 us of a call, which for a single token is four times the kernel.  The
 // entry points of libvcattn.so come in as addresses (bind), from the handle
 // that the ctypes binding has loaded.
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <memory>
+#include <mutex>
 #include <optional>
 #include <sstream>
 #include <string>
+#include <vector>
 
 #include "vcattn.h"
 
@@ -275,15 +280,60 @@ Tensor matmul_blocks(const Library& lib, const Tensor& a, const Tensor& sa, int6
 }
 
 // ---- packed_attention -------------------------------------------------------------
-// What a call needs of a plan.
+// What a call needs of a plan.  It owns the records on the device.
 struct PackedCall {
   int heads, kv_heads;
   int64_t total_q, total_k, head_dim;
   bool causal;
-  uintptr_t work;   // vcattn_packed_work
+  vcattn_packed_work work;   // points into `records`
   size_t workspace;
-  int device;       // index, -1 for a plan on the CPU
+  Tensor records;
 };
+
+// Records that a captured graph reads at each replay.  The graph's end may be
+// seen on a thread that must not call CUDA, so they are let go by a later call.
+struct Ended {
+  std::mutex m;
+  std::vector<Tensor> records;
+  std::atomic<bool> any{false};
+};
+Ended& ended() {
+  static Ended* e = new Ended;   // (graphs may end after this library's statics)
+  return *e;
+}
+void CUDART_CB graph_ended(void* records) {
+  Ended& e = ended();
+  const std::lock_guard<std::mutex> hold(e.m);
+  e.records.push_back(std::move(*static_cast<Tensor*>(records)));
+  delete static_cast<Tensor*>(records);
+  e.any = true;
+}
+void drop_ended() {
+  Ended& e = ended();
+  if (!e.any) return;
+  std::vector<Tensor> gone;
+  const std::lock_guard<std::mutex> hold(e.m);
+  gone.swap(e.records);
+  e.any = false;
+}
+
+// The records stay what they are until the work on `stream` that reads them is
+// done, also if the plan is dropped before: their memory is not handed out
+// again while that stream has not passed this call, and a graph that captures
+// the call owns them.
+void keep_records(const Tensor& records, const c10::cuda::CUDAStream& stream) {
+  drop_ended();
+  c10::cuda::CUDACachingAllocator::recordStream(records.storage().data_ptr(), stream);
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  cudaGraph_t graph = nullptr;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream.stream(), &status, nullptr, &graph));
+  if (status != cudaStreamCaptureStatusActive) return;
+  cudaUserObject_t object = nullptr;
+  auto held = std::make_unique<Tensor>(records);
+  C10_CUDA_CHECK(cudaUserObjectCreate(&object, held.get(), graph_ended, 1, cudaUserObjectNoDestructorSync));
+  held.release();
+  C10_CUDA_CHECK(cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove));
+}
 
 constexpr const char* kPackedCall = "vcattn packed call";
 
@@ -299,7 +349,7 @@ Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, co
   CHECK_VALUE((st == at::kBFloat16 || st == at::kHalf) && k.scalar_type() == st && v.scalar_type() == st,
               "q, k, v must share bfloat16 or float16, got ", st, ", ", k.scalar_type(), ", ", v.scalar_type());
   const at::Device dev = q.device();
-  CHECK_VALUE(k.device() == dev && v.device() == dev && dev.index() == p.device,
+  CHECK_VALUE(k.device() == dev && v.device() == dev && dev == p.records.device(),
               "q, k, v and the plan must be on one device");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(p.head_dim));
   CHECK_VALUE(s > 0.0 && s < 1e30, "scale must be positive and finite, got ", s);
@@ -309,11 +359,13 @@ Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, co
   const vcattn_bhnd vo = bhnd(out);
   Tensor ws;
   if (p.workspace > 0) ws = at::empty_strided({static_cast<int64_t>(p.workspace)}, {1}, q.options().dtype(at::kByte));
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(dev.index());
+  keep_records(p.records, stream);
   lib.status(lib.attn_packed(&vq.v, &vk.v, &vv.v, dtype_code(st), p.heads, p.kv_heads, static_cast<int>(p.total_q),
                                  static_cast<int>(p.total_k), static_cast<int>(p.head_dim),
-                                 reinterpret_cast<const vcattn_packed_work*>(p.work), p.causal ? 1 : 0,
+                                 &p.work, p.causal ? 1 : 0,
                                  static_cast<float>(s), &vo, p.workspace ? ws.data_ptr() : nullptr, p.workspace,
-                                 stream_of(q)),
+                                 stream.stream()),
                "vcattn_attn_packed");
   return out;
 }
@@ -352,8 +404,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   // (a capsule: a registered class could not be registered again by a second copy)
   m.def("packed_call", [](int heads, int kv_heads, int64_t total_q, int64_t total_k, int64_t head_dim, bool causal,
-                          uintptr_t work, size_t workspace, int device) {
-    return py::capsule(new PackedCall{heads, kv_heads, total_q, total_k, head_dim, causal, work, workspace, device}, kPackedCall,
-                       [](PyObject* c) { delete static_cast<PackedCall*>(PyCapsule_GetPointer(c, kPackedCall)); });
+                          uintptr_t work, size_t workspace, const Tensor& records) {
+    drop_ended();
+    return py::capsule(new PackedCall{heads, kv_heads, total_q, total_k, head_dim, causal,
+                                      *reinterpret_cast<const vcattn_packed_work*>(work), workspace, records},
+                       kPackedCall, [](PyObject* c) { delete static_cast<PackedCall*>(PyCapsule_GetPointer(c, kPackedCall)); });
   });
 }

@@ -66,7 +66,7 @@ class PackedPlan:
     joins: Tuple[torch.Tensor, ...]   # and of vcattn_packed_join records
     work: N.PackedWork                # the lists for the C ABI
     workspace_bytes: int              # partial results of one call
-    call: object                      # the same for the host extension
+    call: object                      # the same for the host extension, which keeps the records while a call reads them
 
     @property
     def device(self) -> torch.device:
@@ -182,13 +182,12 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
     need = sum(m[2] * hs * shape.rows * (head_dim + 2) * 4 for m, (_, _, hs, shape) in zip(made, lists))
     # one upload for all records
     host = np.concatenate([m[i] for i in (0, 1) for m in made])
-    recs = torch.from_numpy(host).to(dev).split([len(m[i]) for i in (0, 1) for m in made])
+    records = torch.from_numpy(host).to(dev)
+    recs = records.split([len(m[i]) for i in (0, 1) for m in made])
     work = N.PackedWork(tuple(r.data_ptr() for r in recs[:3]), tuple(r.data_ptr() for r in recs[3:]),
                         tuple(len(r) for r in recs[:3]), tuple(len(r) for r in recs[3:]), tuple(m[2] for m in made))
     tq, tk = int(ql.sum()), int(kl.sum())
-    index = recs[0].device.index
-    call = host_ops().packed_call(heads, kv_heads, tq, tk, head_dim, bool(causal), ctypes.addressof(work), need,
-                                 -1 if index is None else index)
+    call = host_ops().packed_call(heads, kv_heads, tq, tk, head_dim, bool(causal), ctypes.addressof(work), need, records)
     return PackedPlan(heads, kv_heads, head_dim, bool(causal), tq, tk, recs[:3], recs[3:], work, need, call)
 
 
