@@ -292,7 +292,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(kWarps * 32) attn_packed_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   grid_release();
-  const PackedTile t = a.tiles[blockIdx.x / a.Hk];   // longest first, over all heads
+  const PackedTile t = load_tile(a, blockIdx.x / a.Hk, a.G);   // longest first, over all heads
   const int kvh = blockIdx.x % a.Hk;
   const int tid = threadIdx.x, warp = tid >> 5;
   const uint32_t s0 = smem_addr(smem);
@@ -338,7 +338,7 @@ template <int DT, int D, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, STAGES == 2 ? 3 : 2) attn_packed_few_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   grid_release();
-  const PackedTile t = a.tiles[blockIdx.x / a.Hk];   // longest first, over all heads
+  const PackedTile t = load_tile(a, blockIdx.x / a.Hk, a.G);   // longest first, over all heads
   const int kvh = blockIdx.x % a.Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * STAGES * 2 * kFewTile<D>;
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, STAGES == 2 ? 3 : 2) attn_packed_
 template <int DT, int D, int R>
 __global__ void __launch_bounds__(256) attn_packed_join_kernel(const PackedArgs a, int heads, int G) {
   grid_wait();   // the parts
-  const PackedJoin jn = a.joins[blockIdx.x / (R / 8)];
+  const PackedJoin jn = load_join(a, blockIdx.x / (R / 8), G);
   const int row = (blockIdx.x % (R / 8)) * 8 + (threadIdx.x >> 5), head = blockIdx.y, lane = threadIdx.x & 31;
   const int r = jn.r0 + row, tok = r / G;
   if (tok >= jn.lq || jn.q0 + tok >= a.Tq) return;
@@ -608,6 +608,7 @@ VCATTN_API int vcattn_attn_packed(const vcattn_bhnd* q, const vcattn_bhnd* k, co
     x.joins = reinterpret_cast<const PackedJoin*>(work->joins[i]);
     x.n_tiles = work->n_tiles[i];
     x.n_joins = work->n_joins[i];
+    x.slots = work->slots[i];
     const size_t rows = static_cast<size_t>(work->slots[i]) * kListRows[i] * (i == 2 ? Hq : Hk);
     x.part_o = ws;
     x.part_ml = ws + rows * D;

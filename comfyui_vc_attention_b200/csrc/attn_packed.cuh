@@ -30,7 +30,7 @@ struct PackedArgs {
   int64_t qsh, qsn, ksh, ksn, vsh, vsn, osh, osn;   // strides in elements over heads and rows
   const PackedTile* tiles;
   const PackedJoin* joins;
-  int n_tiles, n_joins;
+  int n_tiles, n_joins, slots;
   int Hq, Hk, G, D;
   int Tq, Tk;      // rows of the packed buffers: no tile reads or writes past them
   int causal;
@@ -46,6 +46,28 @@ constexpr int kPackedFewRows = 16;
 constexpr int kPackedRows = 64;
 constexpr int kPackedWideRows = 256;
 constexpr int kListRows[3] = {kPackedFewRows, kPackedRows, kPackedWideRows};
+
+// A record as the kernels use it: empty (no row, no key) if it points before the
+// buffers or outside the workspace, or if its row and key numbers leave 31 bits
+// (rows and keys past Tq and Tk are left out where they are read and written).
+__device__ __forceinline__ bool fits31(int64_t n) { return n < (int64_t{1} << 31) - kPackedWideRows; }
+__device__ __forceinline__ PackedTile load_tile(const PackedArgs& a, int i, int group) {
+  PackedTile t = a.tiles[i];
+  const int64_t rows = static_cast<int64_t>(t.lq) * group;
+  if ((t.q0 | t.lq | t.k0 | t.lk | t.r0 | t.kb) < 0 || t.slot >= a.slots || t.r0 >= rows || !fits31(rows) ||
+      !fits31(static_cast<int64_t>(t.q0) + t.lq) || !fits31(static_cast<int64_t>(t.k0) + t.lk))
+    return PackedTile{0, 0, 0, 0, 0, 0, 0, -1};
+  t.ke = min(t.ke, min(t.lk, max(0, a.Tk - t.k0)));
+  return t;
+}
+__device__ __forceinline__ PackedJoin load_join(const PackedArgs& a, int i, int group) {
+  const PackedJoin j = a.joins[i];
+  if ((j.q0 | j.lq | j.r0 | j.slot0 | j.pieces) < 0 || static_cast<int64_t>(j.slot0) + j.pieces > a.slots ||
+      !fits31(static_cast<int64_t>(j.lq) * group) || j.r0 >= static_cast<int64_t>(j.lq) * group ||
+      !fits31(static_cast<int64_t>(j.q0) + j.lq))
+    return PackedJoin{0, 0, 0, 0, 0, {0, 0, 0}};
+  return j;
+}
 
 cudaError_t launch_attn_packed_tc(const PackedArgs& a, int dtype, cudaStream_t st);
 

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int head = blockIdx.x % a.Hq;
   grid_release();
   if (tid == 0) {
-    sm.t = a.tiles[blockIdx.x / a.Hq];
+    sm.t = load_tile(a, blockIdx.x / a.Hq, 1);
     sm.abort = 0;
     sm.bad = 0;
     mbar_init(&sm.q_full, 1);

@@ -385,8 +385,9 @@ VCATTN_API int vcattn_matmul_blocks(const uint8_t* a8, int64_t lda, const float*
  * head, row = token.  Every query row belongs to one tile, or to the tiles of
  * one join where its keys are split over several; those write `slots` partial
  * results that the joins add up in key order.  kb of a split: a multiple of 64
- * (128 in list 2).  Records that point past Tq or Tk are cut there.  Bounded
- * waits report through vcattn_attn_status as 500 + site. */
+ * (128 in list 2).  Records that point past Tq or Tk are cut there; one with a
+ * negative row or key number, or with partial results outside `slots`, is
+ * passed over.  Bounded waits report through vcattn_attn_status as 500 + site. */
 typedef struct vcattn_packed_tile {
   int32_t q0, lq;   /* first query row in the packed buffer, queries   */
   int32_t k0, lk;   /* first key row, keys                             */
