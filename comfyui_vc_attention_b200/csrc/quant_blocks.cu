@@ -8,8 +8,9 @@
 // maximum is taken on the 16-bit pairs.  Both quotients are Markstein's
 // correction of a product with the reciprocal (see DivBy), so the scales and
 // codes are those of IEEE divisions; the one of x / s runs on packed fp32
-// pairs.  Bound by HBM, the elements read once: 16384 x 14336 bf16 in 116-132 us
-// (5.4-6.1 TB/s), square blocks of 14336 x 5376 in 44 us (5.2 TB/s).
+// pairs, scaled up first in blocks of tiny values (kDivMin).  Bound by HBM, the
+// elements read once: 16384 x 14336 bf16 in 116-132 us (5.4-6.1 TB/s), square
+// blocks of 14336 x 5376 in 44 us (5.2 TB/s).
 #include <string>
 
 #include "kernels.cuh"
@@ -38,6 +39,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+
+// The correction's remainder x - q0 s is a multiple of ulp(q0) ulp(s).  Codes
+// other than 0 have quotients of 2^-10 and more, so from this scale on that is
+// 2^-147 or more and the remainder exact; below it (wrong codes next to ties
+// from a maximum of 2^-99 down) x and s are multiplied by 2^64 first, exactly.
+// (The division itself took 3.4 times as long on blocks of zeros.)
+constexpr float kDivMin = 0x1p-90f, kDivUp = 0x1p64f;
 
 // Eight consecutive columns as loaded: 16-bit pairs, or fp32.
 template <int DT> struct Cols8 {
@@ -70,6 +78,18 @@ template <int DT> struct Cols8 {
       y = f.y;
     }
   }
+  // All columns times kDivUp.  (Blocks of f16 that small hold zeros alone.)
+  __device__ __forceinline__ void scale_up() {
+    if constexpr (DT == VCATTN_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x, y;
+        pair(i, x, y);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x * kDivUp, y * kDivUp);
+        u[i] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    }
+  }
   __device__ __forceinline__ void load(const void* p) {
     const uint4 v = *reinterpret_cast<const uint4*>(p);
     u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
@@ -93,6 +113,10 @@ template <> struct Cols8<VCATTN_DTYPE_F32> {
   __device__ __forceinline__ void pair(int i, float& x, float& y) const {
     x = v[2 * i];
     y = v[2 * i + 1];
+  }
+  __device__ __forceinline__ void scale_up() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= kDivUp;
   }
   __device__ __forceinline__ void load(const void* p) {
     const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
@@ -121,6 +145,18 @@ __device__ __forceinline__ float block_scale(float amax) {
   const float q0 = __fmul_rn(amax, y);
   const float q = __fmaf_rn(__fmaf_rn(-q0, kE4M3Max, amax), y, q0);
   return amax < INFINITY ? q : amax;
+}
+
+// The divisor of a block's values and its reciprocal.
+template <int DT, int N>
+__device__ __forceinline__ float divisor(float s, Cols8<DT> (&v)[N], float& y) {
+  if (s < kDivMin) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) v[u].scale_up();
+    s *= kDivUp;
+  }
+  y = __frcp_rn(s);
+  return s;
 }
 
 __device__ __forceinline__ uint32_t codes2(float lo, float hi) {
@@ -186,8 +222,9 @@ __global__ void __launch_bounds__(kThreads) quant_rows_blocks_kernel(const Quant
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (seg >= a.segs) return;
-  const float s = block_scale(m), y = __frcp_rn(s);
+  float s = block_scale(m), y;
   if (l == 0) a.scale[row * a.ssm + blk * a.ssk] = s;
+  s = divisor(s, v, y);
 #pragma unroll
   for (int u = 0; u < kChunks; ++u) store_codes<DT>(a, row, blk * kBlk + (u * kLanes + l) * 8, v[u], s, y);
 }
@@ -212,8 +249,9 @@ __global__ void __launch_bounds__(kThreads) quant_square_blocks_kernel(const Qua
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) m = max_nan(m, wmax[w]);
-  const float s = block_scale(m), y = __frcp_rn(s);
+  float s = block_scale(m), y;
   if (threadIdx.x == 0) a.scale[mb * a.ssm + blk * a.ssk] = s;
+  s = divisor(s, v, y);
 #pragma unroll
   for (int u = 0; u < 8; ++u)
     if (r0 + 16 * u < a.M) store_codes<DT>(a, r0 + 16 * u, c, v[u], s, y);
