@@ -7,7 +7,9 @@ the objects link into ``comfyui_vc_attention_b200/libvcattn.so``.  The library
 exports only the C ABI of ``include/vcattn.h``; it does not link against torch.
 The host side of the block operators (``csrc/host_ops.cpp``) is a Python
 extension over torch's tensors, ``vc_attention/_host_ops.so``, that calls that
-ABI.  A source is recompiled when it, or any header, is newer than its object.
+ABI; without torch only the library is built.  A source is recompiled when it,
+or any header, is newer than its object, the extension also when torch, Python
+or the command changes.
 """
 
 from __future__ import annotations
@@ -55,13 +57,15 @@ def _compile(src: str, obj: str, extra) -> str:
 
 
 def _host_ops(force: bool) -> None:
-    src = os.path.join(CSRC, "host_ops.cpp")
-    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "vcattn.h")))
-    if not force and os.path.exists(HOST_OPS) and os.path.getmtime(HOST_OPS) >= newest:
+    try:
+        import torch
+    except ImportError as e:
+        print(f"torch cannot be imported ({e}): {os.path.basename(HOST_OPS)}, the host side of the block operators, "
+              f"is not built", file=sys.stderr)
         return
     import sysconfig
 
-    import torch
+    src = os.path.join(CSRC, "host_ops.cpp")
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     inc = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
@@ -69,10 +73,20 @@ def _host_ops(force: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_host_ops",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in inc], src,
            "-o", HOST_OPS + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    # what the extension was built with and for
+    made = "\n".join([torch.__version__, sys.version, *cmd])
+    stamp = os.path.join(BUILD, "host_ops.txt")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "vcattn.h")))
+    if not force and os.path.exists(HOST_OPS) and os.path.getmtime(HOST_OPS) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == made:
+                return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for host_ops.cpp:\n{r.stderr}\n{r.stdout}")
     os.replace(HOST_OPS + ".tmp", HOST_OPS)
+    with open(stamp, "w") as f:
+        f.write(made)
 
 
 def build(force: bool = False, jobs: int = 0, verbose: bool = False, extra=()) -> str:
@@ -95,13 +109,13 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False, extra=()) -
                 msg = f.result()
                 if verbose and msg.strip():
                     print(f"[{os.path.basename(futs[f])}]\n{msg}", file=sys.stderr)
-        host.result()
-    if todo or not os.path.exists(LIB):
+    if todo or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(map(os.path.getmtime, objs), default=0.0):
         cmd = [nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", LIB + ".tmp"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}\n{r.stdout}")
         os.replace(LIB + ".tmp", LIB)
+    host.result()   # (after the link: the library does not depend on it)
     return LIB
 
 
