@@ -5,6 +5,7 @@
 // 16 us of a call, which for a single token is four times the kernel.  The
 // entry points of libvcattn.so come in as addresses (bind), from the handle
 // that the ctypes binding has loaded.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -61,12 +62,19 @@ void need_cuda(bool cuda, const char* fn) {
   if (!cuda) throw std::runtime_error(text(fn, " needs CUDA tensors (this build has no CPU path)"));
 }
 
-// The operators have no backward pass: say so instead of cutting the graph.
-template <typename... T> void refuse_grad(const char* fn, const T&... t) {
-  if (at::GradMode::is_enabled() && (t.requires_grad() || ...))
+// The operators have no derivatives, backward or forward (a tangent sits on the
+// tensor whatever the gradient mode): say so instead of dropping them.
+void refuse_one(const char* fn, const Tensor& t) {
+  if (!t.defined()) return;
+  if (t.requires_grad() && at::GradMode::is_enabled())
     throw std::runtime_error(text(fn, " has no backward pass: call it under torch.no_grad() or on detached tensors"));
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
+    throw std::runtime_error(text(fn, " has no forward derivative: call it on detached tensors"));
 }
-bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+void refuse_one(const char* fn, const OptTensor& t) {
+  if (t.has_value()) refuse_one(fn, *t);
+}
+template <typename... T> void refuse_grad(const char* fn, const T&... t) { (refuse_one(fn, t), ...); }
 
 int dtype_code(at::ScalarType t) {
   switch (t) {
@@ -133,9 +141,7 @@ constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;
 std::tuple<Tensor, Tensor> qk_norm_rope(const Library& lib, const Tensor& q, const Tensor& k, const OptTensor& cos_in, const OptTensor& sin_in,
                                         const OptTensor& q_weight, const OptTensor& k_weight, const std::string& layout,
                                         double eps, bool norm, const OptTensor& out_q, const OptTensor& out_k) {
-  refuse_grad("qk_norm_rope", q, k);
-  if (at::GradMode::is_enabled() && (wants_grad(cos_in) || wants_grad(sin_in) || wants_grad(q_weight) || wants_grad(k_weight)))
-    throw std::runtime_error("qk_norm_rope has no backward pass: call it under torch.no_grad() or on detached tensors");
+  refuse_grad("qk_norm_rope", q, k, cos_in, sin_in, q_weight, k_weight, out_q, out_k);
   need_cuda(q.is_cuda() && k.is_cuda(), "qk_norm_rope");
   CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3),
               "q and k must be (B, Hq, N, D) and (B, Hk, N, D), got ", q.sizes(), ", ", k.sizes());
@@ -237,8 +243,7 @@ Tensor code_rows(const Tensor& c, const Tensor& s, int64_t rows, int64_t want, c
 
 Tensor matmul_blocks(const Library& lib, const Tensor& a, const Tensor& sa, int64_t a_rows, const Tensor& b, const Tensor& sb, int64_t b_rows,
                      const OptTensor& bias_in, const py::object& dtype, const OptTensor& out_in) {
-  refuse_grad("matmul_blocks", sa, sb);
-  if (bias_in.has_value()) refuse_grad("matmul_blocks", *bias_in);
+  refuse_grad("matmul_blocks", a, sa, b, sb, bias_in, out_in);
   int64_t lda = 0, ldb = 0;
   c10::cuda::OptionalCUDAGuard guard;
   if (a.is_cuda()) guard.set_device(a.device());
@@ -339,7 +344,7 @@ constexpr const char* kPackedCall = "vcattn packed call";
 
 Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, const Tensor& v, const PackedCall& p, std::optional<double> scale,
                         const OptTensor& out_in) {
-  refuse_grad("packed_attention", q, k, v);
+  refuse_grad("packed_attention", q, k, v, out_in);
   need_cuda(q.is_cuda() && k.is_cuda() && v.is_cuda(), "packed_attention");
   const std::array<int64_t, 4> wq{1, p.heads, p.total_q, p.head_dim}, wk{1, p.kv_heads, p.total_k, p.head_dim};
   CHECK_VALUE(q.sizes() == at::IntArrayRef(wq) && k.sizes() == at::IntArrayRef(wk) && v.sizes() == at::IntArrayRef(wk),
