@@ -5,6 +5,7 @@
 // 16 us of a call, which for a single token is four times the kernel.  The
 // entry points of libvcattn.so come in as addresses (bind), from the handle
 // that the ctypes binding has loaded.
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAException.h>
@@ -106,6 +107,23 @@ View view(const Tensor& t) {
   return {bhnd(c), c};
 }
 
+// Outputs that the caller gives may not share memory with a tensor that the
+// kernel reads at other places, or at other times, than it writes.  (Two views
+// that interleave, as those of a fused projection, are told apart only where
+// they start at the same element.)
+bool same_start(const Tensor& x, const Tensor& y) { return x.numel() > 0 && y.numel() > 0 && x.data_ptr() == y.data_ptr(); }
+void apart(const Tensor& out, const Tensor& in, const char* what, const char* other) {
+  const at::MemOverlapStatus o = at::get_overlap_status(out, in);
+  CHECK_VALUE(o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial && !same_start(out, in), what,
+              " overlaps ", other);
+}
+// The same for the input that it may be written over.
+void in_place_or_apart(const Tensor& out, const Tensor& in, const char* what, const char* other) {
+  CHECK_VALUE(at::get_overlap_status(out, in) != at::MemOverlapStatus::Partial &&
+                  (!same_start(out, in) || out.strides() == in.strides()),
+              what, " overlaps a part of ", other);
+}
+
 // `out` checked against its input, or a new buffer with its dimensions in the
 // input's order in memory (the ComfyUI (B, N, H*D) path stays token-major).
 Tensor out_rows(const OptTensor& out, const Tensor& x, const char* what) {
@@ -184,6 +202,15 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Library& lib, const Tensor& q, con
   const float* kw = weight(k_weight, d, dev, "k_weight", wk);
   c10::cuda::CUDAGuard guard(dev);
   const Tensor oq = out_rows(out_q, q, "out[0]"), ok = out_rows(out_k, k, "out[1]");
+  if (out_q.has_value()) {
+    in_place_or_apart(oq, q, "out[0]", "q");
+    apart(oq, k, "out[0]", "k");
+  }
+  if (out_k.has_value()) {
+    in_place_or_apart(ok, k, "out[1]", "k");
+    apart(ok, q, "out[1]", "q");
+    apart(ok, oq, "out[1]", "out[0]");
+  }
   const View vq = view(q), vk = view(k);
   const vcattn_bhnd wq_out = bhnd(oq), wk_out = bhnd(ok);
   lib.status(lib.qk_norm_rope(&vq.v, &vk.v, dt, static_cast<int>(b), static_cast<int>(q.size(1)),
@@ -269,6 +296,8 @@ Tensor matmul_blocks(const Library& lib, const Tensor& a, const Tensor& sa, int6
                     (n <= 1 || out.stride(1) == 1) && (m <= 1 || out.stride(0) >= n),
                 "out must be (", m, ", ", n, ") ", st, " on ", dev, " with contiguous columns");
     if (m > 1) ldo = out.stride(0);
+    for (const Tensor* t : {&a, &sa, &b, &sb}) apart(out, *t, "out", "an operand");
+    if (bias.defined()) apart(out, bias, "out", "the bias");
   } else {
     out = at::empty_strided({m, n}, {ldo, 1}, a.options().dtype(st));
   }
@@ -360,6 +389,11 @@ Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, co
   CHECK_VALUE(s > 0.0 && s < 1e30, "scale must be positive and finite, got ", s);
   c10::cuda::CUDAGuard guard(dev);
   const Tensor out = out_rows(out_in, q, "out");
+  if (out_in.has_value()) {
+    in_place_or_apart(out, q, "out", "q");
+    apart(out, k, "out", "k");
+    apart(out, v, "out", "v");
+  }
   const View vq = view(q), vk = view(k), vv = view(v);
   const vcattn_bhnd vo = bhnd(out);
   Tensor ws;
