@@ -405,11 +405,43 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && nh > 0) ok = warp_wait(&sm.o_full[h], 0, abort, status, 9);
     tc_fence_after();
     const float l = l0 + l1;
-    const bool bad = *static_cast<volatile int*>(&sm.bad) != 0;
+    const bool bad = __any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.bad) != 0);
     const bool part = t.slot >= 0;
     const float inv = part ? 1.f : l != 0.f ? __fdiv_rn(1.f, l) : 0.f;   // (l is NaN where a score was)
     const int64_t prow = (static_cast<int64_t>(t.slot) * a.Hq + head) * (2 * kHalf) + h * kHalf + row;
     if (__all_sync(0xffffffffu, ok && *abort == 0)) {
+      if (bad && nh > 0) {
+        // The infinite and NaN values of the edge tiles, for the rows that see
+        // them.  All of the row before any of it is written: out may be q.
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + head * a.qsh + static_cast<int64_t>(t.q0 + tok) * a.qsn;
+        const uint16_t* k0 = static_cast<const uint16_t*>(a.k) + (head / a.G) * a.ksh;
+        const uint16_t* v0 = static_cast<const uint16_t*>(a.v) + (head / a.G) * a.vsh;
+        const int end = live ? min(lim, a.Tk - t.k0) : 0;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          __syncwarp();
+          float o[32];
+          tmem_ld32(to + 32 * c, o);
+          tmem_ld_wait();
+          reg_fence(o);
+          for (int key = max(t.kb, row_limit(t, a.causal, t.r0)); key < end; ++key) {
+            const uint16_t* v = v0 + static_cast<int64_t>(t.k0 + key) * a.vsn + 32 * c;
+            bool hit = false;
+            for (int e = 0; e < 32; ++e) hit |= not_finite<DT>(v[e]);
+            if (!hit) continue;
+            const uint16_t* k = k0 + static_cast<int64_t>(t.k0 + key) * a.ksn;
+            float s = 0.f;
+            for (int e = 0; e < D; ++e) s = fmaf(value16<DT>(q[e]), value16<DT>(k[e]), s);
+            const float p = ex2(fmaf(s, sl2, m == -INFINITY ? 0.f : -m));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (not_finite<DT>(v[e])) o[e] = fmaf(p, value16<DT>(v[e]), o[e]);
+          }
+          __syncwarp();
+          tmem_st32(to + 32 * c, o);
+        }
+        tmem_st_wait();
+      }
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         __syncwarp();   // the lanes part below, and the load of tensor memory is one of the whole warp
@@ -422,24 +454,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (nh == 0 || lim <= t.kb) {   // no key of this range
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        }
-        if (live && bad) {
-          // the infinite and NaN values of the edge tiles, for the rows that see them
-          const uint16_t* q = static_cast<const uint16_t*>(a.q) + head * a.qsh + static_cast<int64_t>(t.q0 + tok) * a.qsn;
-          const int kvh = head / a.G;
-          for (int key = max(t.kb, row_limit(t, a.causal, t.r0)); key < min(lim, a.Tk - t.k0); ++key) {
-            const uint16_t* v = static_cast<const uint16_t*>(a.v) + kvh * a.vsh + static_cast<int64_t>(t.k0 + key) * a.vsn + 32 * c;
-            bool hit = false;
-            for (int e = 0; e < 32; ++e) hit |= not_finite<DT>(v[e]);
-            if (!hit) continue;
-            const uint16_t* k = static_cast<const uint16_t*>(a.k) + kvh * a.ksh + static_cast<int64_t>(t.k0 + key) * a.ksn;
-            float s = 0.f;
-            for (int e = 0; e < D; ++e) s = fmaf(value16<DT>(q[e]), value16<DT>(k[e]), s);
-            const float p = ex2(fmaf(s, sl2, m == -INFINITY ? 0.f : -m));
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (not_finite<DT>(v[e])) o[e] = fmaf(p, value16<DT>(v[e]), o[e]);
-          }
         }
         if (live && part) {
           float4* po = reinterpret_cast<float4*>(a.part_o + prow * D + 32 * c);

@@ -61,3 +61,20 @@ def test_product_outputs_that_overlap():
     with pytest.raises(ValueError, match="overlaps"):
         matmul_blocks(a, b, y[0], torch.float32, out=y)
     matmul_blocks(a, b, out=store[40 * 256:40 * 256 + 40 * 128 * 2].view(torch.bfloat16).view(40, 128))
+
+
+@pytest.mark.parametrize("d,lq,lk", [(128, 300, 300), (64, 300, 300), (128, 270, 5000), (128, 30, 90), (64, 4, 700)])
+def test_attention_over_q_with_infinite_values(d, lq, lk):
+    """Values that are infinite behind the causal mask of some rows, in channels of several
+    parts of the row: the output over q has the bits of the output beside it."""
+    from comfyui_vc_attention_b200.vc_attention import packed_attention, packed_plan
+    g = torch.Generator("cuda").manual_seed(d + lk)
+    q, k, v = (torch.randn(1, 8, n, d, generator=g, device="cuda").to(torch.bfloat16) for n in (lq, lk, lk))
+    for i, c in enumerate((3, 40, d - 1, 17, 33)):
+        v[:, :, lk - lq + (i + 1) * lq // 7, c] = float("inf") if i % 2 else -float("inf")
+        v[:, :, lk - lq + (i + 1) * lq // 7, (c + 32) % d] = float("inf")
+    plan = packed_plan([lq], [lk], heads=8, head_dim=d, causal=True)
+    want = packed_attention(q, k, v, plan)
+    assert want.isinf().any() and torch.isfinite(want).any()
+    got = packed_attention(q, k, v, plan, out=q)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16))
