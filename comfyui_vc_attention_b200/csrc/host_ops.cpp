@@ -124,6 +124,12 @@ void in_place_or_apart(const Tensor& out, const Tensor& in, const char* what, co
               what, " overlaps a part of ", other);
 }
 
+// Tells autograd that `t` has new contents, so that a backward pass which needs
+// the old ones refuses instead of using these.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // `out` checked against its input, or a new buffer with its dimensions in the
 // input's order in memory (the ComfyUI (B, N, H*D) path stays token-major).
 Tensor out_rows(const OptTensor& out, const Tensor& x, const char* what) {
@@ -219,6 +225,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Library& lib, const Tensor& q, con
                                   rot ? static_cast<const float*>(sin.data_ptr()) : nullptr, tsb, tsn,
                                   static_cast<int>(rot), flags, static_cast<float>(eps), &wq_out, &wk_out, stream_of(q)),
                "vcattn_qk_norm_rope");
+  if (out_q.has_value()) written(oq);
+  if (out_k.has_value()) written(ok);
   return {oq, ok};
 }
 
@@ -310,6 +318,7 @@ Tensor matmul_blocks(const Library& lib, const Tensor& a, const Tensor& sa, int6
                                    bias.defined() ? static_cast<const float*>(bias.data_ptr()) : nullptr, out.data_ptr(), odt,
                                    ldo, need ? ws.data_ptr() : nullptr, need, stream_of(a)),
                "vcattn_matmul_blocks");
+  if (out_in.has_value()) written(out);
   return out;
 }
 
@@ -406,6 +415,7 @@ Tensor packed_attention(const Library& lib, const Tensor& q, const Tensor& k, co
                                  static_cast<float>(s), &vo, p.workspace ? ws.data_ptr() : nullptr, p.workspace,
                                  stream.stream()),
                "vcattn_attn_packed");
+  if (out_in.has_value()) written(out);
   return out;
 }
 

@@ -78,3 +78,28 @@ def test_attention_over_q_with_infinite_values(d, lq, lk):
     assert want.isinf().any() and torch.isfinite(want).any()
     got = packed_attention(q, k, v, plan, out=q)
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+def test_autograd_sees_what_was_written():
+    """A backward pass that needs a tensor which an operator has overwritten refuses."""
+    from comfyui_vc_attention_b200.vc_attention import (matmul_blocks, packed_attention, packed_plan, qk_norm_rope,
+                                                        quantize_blocks)
+    cos, sin = _tables(20, 64)
+    plan = packed_plan([20], heads=2, head_dim=64)
+    a8 = quantize_blocks(torch.randn(10, 128, device="cuda"))
+    b8 = quantize_blocks(torch.randn(256, 128, device="cuda"), 128)
+    calls = [lambda x: qk_norm_rope(x, x.clone(), cos, sin, out=(x, x.clone())),
+             lambda x: qk_norm_rope(x.clone(), x, cos, sin, out=(x.clone(), x)),
+             lambda x: packed_attention(x, x.clone(), x.clone(), plan, out=x),
+             lambda x: matmul_blocks(a8, b8, dtype=x.dtype, out=x.view(10, 256))]
+    for call in calls:
+        w = torch.ones(1, 2, 20, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        y = w * 1
+        z = (y * y).sum()
+        call(y.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    with torch.inference_mode():
+        x = torch.ones(1, 2, 20, 64, device="cuda", dtype=torch.bfloat16)
+        for call in calls:
+            call(x)
