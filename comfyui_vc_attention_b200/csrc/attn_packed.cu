@@ -2,7 +2,7 @@
 // sequences: the rows of a KV head's group share one pass over its keys.
 //
 //   O = softmax(scale q k^T + mask) v,  one pass with a running maximum m and
-//   sum l per row (both fp32):  O <- O 2^(m - m') + P V,  P = 2^(s - m')
+//   sum l per row (both fp32):  O <- O 2^(m - m') + P V,  P = 2^(s - m' + kRaise)
 //
 // A tile is 64 or 16 rows (token, group head) of one sequence and KV head
 // against a range of its keys.  cp.async brings K and V to shared memory; keys
@@ -76,6 +76,12 @@ template <int DT> __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (DT == VCATTN_DTYPE_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
+
+// P is made 2^kRaise times as large, and so are l and O, which cancels in O / l.
+// In bf16 that changes nothing; f16 has steps of 2^-24 below 2^-14, which all
+// the keys behind one of a much larger score would share (65536 keys, 18 nats
+// below the first: 1.4 % of the output), so P uses its range up to 2^15.
+template <int DT> constexpr float kRaise = DT == VCATTN_DTYPE_F16 ? 15.f : 0.f;
 
 template <int D> constexpr int kPitch = D * 2 + 16;   // bytes of a row in shared memory: eight rows start in different banks
 
@@ -181,7 +187,7 @@ template <int DT, int D> struct Rows16 {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];   // a row without a key so far
+    for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i] - kRaise<DT>;   // (a row without a key so far: 0)
     uint32_t pa[KEYS / 16][4];
 #pragma unroll
     for (int n = 0; n < KEYS / 8; ++n) {
