@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -74,12 +75,15 @@ class PackedPlan:
 
 
 def _lengths(x, what) -> np.ndarray:
-    a = np.asarray([int(v) for v in x], dtype=np.int64)
-    if (a < 0).any():
+    try:
+        n = [operator.index(v) for v in x]
+    except TypeError as e:
+        raise TypeError(f"{what} must be whole numbers") from e
+    if any(v < 0 for v in n):
         raise ValueError(f"{what} must not be negative")
-    if a.sum() >= 2 ** 31:
+    if sum(n) >= 2 ** 31:   # (in Python's numbers: in 64 bits the sum may wrap)
         raise ValueError(f"{what} add up to 2^31 rows or more")
-    return a
+    return np.asarray(n, dtype=np.int64)
 
 
 def _pieces(ke: np.ndarray, heads: int, shape: _Shape):
