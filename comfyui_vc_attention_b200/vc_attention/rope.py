@@ -40,7 +40,12 @@ def rope_tables(positions: torch.Tensor, rot_dim: Union[int, Sequence[int]], the
       "yarn":   per channel pair, between no change (more than ``beta_fast``
                 turns over ``original_len`` positions) and "linear" (fewer than
                 ``beta_slow``), with both tables multiplied by
-                ``1 + 0.1 ln(factor)``.
+                ``1 + 0.1 ln(factor)``.  In between the weight is linear in
+                the number of turns, which is the published method's rule.
+                Code that ramps over the channel index instead (between the
+                rounded indices of the two bounds) gives other tables in the
+                middle channels: a checkpoint trained with such tables needs
+                those, passed as cos and sin.
     """
     dims = [int(rot_dim)] if isinstance(rot_dim, int) else [int(r) for r in rot_dim]
     pos = positions if not isinstance(rot_dim, int) else positions.unsqueeze(-1)
