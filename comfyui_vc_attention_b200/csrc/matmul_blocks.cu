@@ -337,8 +337,10 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
 #pragma unroll
       for (int c = 0; c < 64; ++c) acc[c] = 0.f;
       for (int k = pc.k0(); k < pc.k1(a); k += kGroup) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&sm.s_full[g], g_par, abort, status, 4));
-        if (!ok) break;
+        // (The lanes of a warp may learn at different times that a wait was given
+        // up, so none leaves the loop for it: the waits return at once from then
+        // on, and the vote below ends the work.  A vote or a break here costs 8 %.)
+        mbar_wait(&sm.s_full[g], g_par, abort, status, 4);
         const float4 s4 = *reinterpret_cast<const float4*>(scale + g * (BN / 128 * kBM * kGroup));
         warp_arrive(&sm.s_empty[g], lane);
         g ^= 1;
@@ -347,8 +349,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
           if (k + u >= pc.k1(a)) break;
-          // (a lane that gave up keeps step with the others until the next vote; one here costs 2 %)
-          ok = ok && mbar_wait(&sm.t_full[b], b_par, abort, status, 6);
+          mbar_wait(&sm.t_full[b], b_par, abort, status, 6);
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
           b_par ^= b == 0;
         }
       }
-      ok = __all_sync(0xffffffffu, ok && *abort == 0);
+      ok = __all_sync(0xffffffffu, *abort == 0);
       if (!ok) continue;
       if constexpr (SHARE == kCluster) {
         // this rank's sums over the operand stages (every MMA has read them)
