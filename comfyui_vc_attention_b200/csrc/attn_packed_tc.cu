@@ -1,5 +1,6 @@
-// Packed attention on the 5th-generation tensor cores, for query sequences
-// long enough to fill 128-row tiles.
+// Packed attention on the 5th-generation tensor cores, for the sequences whose
+// queries cost more in 64-row register-MMA tiles over a KV head's group (from 17
+// queries on with one query head per KV head, from 33 with four).
 //
 //   O = softmax(scale q k^T + mask) v,  one pass over the keys with a running
 //   reference m and sum l per row (fp32)
@@ -28,9 +29,10 @@
 // look for infinite or NaN values, which enter the product as 0; the rows
 // that see them add their share at the end.
 // Bound by the power cap on long sequences (16384 x 16384, 14 heads x 128:
-// 1.80 ms, 1.07 PFLOP/s, three quarters of the sustained cuBLAS rate; 1.58 ms
-// in short runs, of which 2^x takes 0.13 and the whole softmax 0.23), by item
-// set-up and output on short ones.  Every wait is bounded.
+// 1.82 ms, 1.06 PFLOP/s, three quarters of the sustained cuBLAS rate; 1.58 ms
+// in short runs, of which 2^x takes 0.13 and the whole softmax 0.23; 14 heads x
+// 64 1.38 ms, where the 2^x alone are 0.81), by item set-up and output on short
+// ones (causal prompts of 4097 queries 161 us).  Every wait is bounded.
 #include "attn_packed.cuh"
 
 #include <cuda.h>

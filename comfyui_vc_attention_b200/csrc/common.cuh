@@ -136,7 +136,9 @@ __device__ __forceinline__ float e4m3_row_scale(float amax) {
 // exactly (fma), q = RN(q0 + r y).  It is the correctly rounded quotient
 // whenever x / s and the residual stay in the normal range.  The E4M3 codes
 // only use quotients up to 448, and any quotient below 2^-10 becomes code 0
-// whatever its last bit, so the codes equal those of an IEEE division.
+// whatever its last bit, so the codes equal those of an IEEE division for
+// scales of 2^-90 and more (below, the residual of a small quotient may be
+// rounded to the subnormal step).
 struct DivBy {
   float s, y;
   __device__ __forceinline__ explicit DivBy(float s_) : s(s_), y(0.f) {

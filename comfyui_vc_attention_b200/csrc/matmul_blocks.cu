@@ -11,8 +11,8 @@
 //   warps 2-3    sa * sb of four k-blocks at a time, in two groups in shared
 //                memory, the next group's loads in flight
 //   warps 4-     promotion and output
-// 16384 x 7168 x 5376: 593 us (2.13 PFLOP/s) in short runs and 670 at the power
-// cap; 523 without the promotion, 410 without the loads (48 KB per k-block and
+// 16384 x 7168 x 5376: 577-593 us (2.1-2.2 PFLOP/s) in short runs and 674 at the
+// power cap; 523 without the promotion, 410 without the loads (48 KB per k-block and
 // SM from L2, 13.5 TB/s over all).  Eight promotion warps of 128 columns whose
 // scales came from global memory took 1050 us.
 #include <cuda.h>
@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(MmCfg<BN>::kThreads, 1)
       }
       if (a.bias != nullptr) {
         // this warp's 64 values, two per lane (one coalesced load each), then
-        // from lane to lane: 64 loads per thread cost 10 us of a 45 us product
+        // from lane to lane: 64 loads per thread cost 8 us (333 x 14336 x 5376,
+        // the same inputs each time: 53 against 45; rotated inputs: 49.6)
         const float b0 = n0 + lane < a.N ? __ldg(a.bias + n0 + lane) : 0.f;
         const float b1 = n0 + 32 + lane < a.N ? __ldg(a.bias + n0 + 32 + lane) : 0.f;
 #pragma unroll

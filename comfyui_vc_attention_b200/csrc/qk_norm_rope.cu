@@ -13,7 +13,8 @@
 // makes them for one token and applies them to its heads, whose rows it has
 // loaded before.  Bound by HBM, every element read once and written once: a
 // 16384-token clip of 56 + 56 heads x 128 bf16 in 154 us interleaved (6.1 TB/s)
-// and 170-180 us in the half layout, whose two chunks per lane take 90 registers.
+// and 182 us in the half layout (170 into the same buffers again and again),
+// whose two chunks per lane take 92 registers.
 #include <string>
 
 #include "kernels.cuh"

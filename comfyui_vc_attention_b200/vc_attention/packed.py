@@ -9,6 +9,10 @@ host numbers, checked here, so no call can read past the buffers) and
 
 Kernels: ``vcattn_attn_packed`` (tcgen05 for sequences of many queries,
 register MMAs over the rows of a KV head's group for few).  Forward only.
+
+A plan may be used on any stream and dropped while its calls still run: the
+records that the kernels read stay until then, and as long as a captured graph
+needs them.
 """
 
 from __future__ import annotations
@@ -200,9 +204,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     """softmax(scale q k^T + mask) v for every sequence of ``plan``.
 
     q: (1, heads, total_q, D), k, v: (1, kv_heads, total_k, D) CUDA bf16 or
-    fp16 views (channels contiguous; others are copied).  scale: positive,
-    default D ** -0.5.  Returns (1, heads, total_q, D) in q's token layout, or
-    writes ``out``.  Scores, statistics and sums are fp32; P is rounded to q's
-    type for the second product.
+    fp16 views (channels contiguous; others are copied), the sequences' rows one
+    after the other.  scale: positive, default D ** -0.5.  Returns (1, heads,
+    total_q, D) in q's token layout, or writes ``out``, which may be q but not
+    overlap k or v.  Scores, statistics and sums are fp32; P is rounded to q's
+    type for the second product (in fp16 to 2^-11 of itself or 2^-36 of the
+    row's largest).
     """
     return host_ops().packed_attention(q, k, v, plan.call, scale, out)
