@@ -44,7 +44,7 @@ def test_plan_dropped_while_another_stream_has_not_run_the_call():
     side, span = torch.cuda.Stream(), _span(plan)
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(200_000_000)          # about 0.1 s
+        torch.cuda._sleep(1_000_000_000)        # about 0.5 s
         got = packed_attention(q, k, v, plan)
     del plan
     gc.collect()
